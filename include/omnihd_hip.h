@@ -683,6 +683,57 @@ int omnihd_radar_merge(const float* raw, int n, int load_dim, const int* sweep_o
                        const double* sweep_consts, const float* pc_range6, float* out10, unsigned char* in_range,
                        void* stream);
 
+/* ------------------------------------------------------------------------------------------
+ * Token operators: rows of a residual stream, their embedding and a teacher's top logits
+ * (no counterpart in the reference's hot path).  Element types are given as codes:
+ * 0 = float32, 1 = bfloat16, 2 = IEEE half; row strides in elements, rows dense within.
+ * None of them synchronises, keeps state or uses atomics on values: results repeat bit for bit.
+ * ---------------------------------------------------------------------------------------- */
+
+/* out[i] = scale * table[ids[i]], out dense [n][dim]; a row of NaN where ids[i] is outside [0, vocab).
+ * ids are int64 (wide_ids = 1) or int32.  table_type == out_type, or table_type = float32.                        */
+int omnihd_token_embed_fwd(const void* ids, int wide_ids, long long n, const void* table, int table_type, long long table_stride,
+                           long long vocab, int dim, float scale, void* out, int out_type, void* stream);
+/* grad[v] = scale * sum of g[i] over the i with ids[i] = v, in increasing order of i, fp32 sums, every row of the dense
+ * [vocab][dim] gradient written.  Ids outside [0, vocab) and those equal to `padding` (-1: none) add nothing.        */
+size_t omnihd_token_embed_bwd_workspace_bytes(long long n, int dim);
+int omnihd_token_embed_bwd(const void* ids, int wide_ids, long long n, const void* g, int out_type, long long g_stride, long long vocab,
+                           int dim, float scale, long long padding, void* grad, int table_type, void* workspace,
+                           size_t workspace_bytes, void* stream);
+
+/* norm(v; w) = v * rsqrt(mean(v^2) + eps) * w over rows of dim <= 16384.
+ *   y given:  x_out = residual_scale * x + gate * norm(y; post),  h_out = norm(x_out before its rounding; next)
+ *             (post NULL: y itself; gate NULL: 1; next NULL: no h_out)
+ *   y NULL:   h_out = norm(x; next)
+ * x, x_out have x_type; y, h_out act_type; x_type == act_type or float32.  gate_kind 0: none; 1: [rows / rows_per_gate][dim],
+ * one row for rows_per_gate rows each; 2: one number a row; 3: as y.  stats (NULL, or 2 floats a row): for the backward. */
+int omnihd_block_join_fwd(const void* x, long long x_stride, int x_type, const void* y, long long y_stride, int act_type,
+                          const void* post, int post_type, const void* gate, int gate_type, int gate_kind, long long gate_stride,
+                          long long rows_per_gate, const void* next, int next_type, float residual_scale, float eps, long long rows,
+                          int dim, void* x_out, void* h_out, float* stats, void* stream);
+/* Gradients of the same inputs (each output may be NULL: not wanted) from dx_out, dh (each may be NULL: zero).  Gradients of
+ * post, next and gate have those arrays' types and are dense; fp32 sums in a fixed order.                              */
+size_t omnihd_block_join_bwd_workspace_bytes(long long rows, int dim, int gate_kind, long long rows_per_gate);
+int omnihd_block_join_bwd(const void* x, long long x_stride, int x_type, const void* y, long long y_stride, int act_type,
+                          const void* post, int post_type, const void* gate, int gate_type, int gate_kind, long long gate_stride,
+                          long long rows_per_gate, const void* next, int next_type, float residual_scale, long long rows, int dim,
+                          const float* stats, const void* dx_out, long long dx_out_stride, const void* dh, long long dh_stride,
+                          void* gx, void* gy, void* g_post, void* g_gate, void* g_next, void* workspace, size_t workspace_bytes,
+                          void* stream);
+
+/* p = softmax of t / temperature over a row's filled slots (ids >= 0), q = softmax of z / temperature over its vocab entries:
+ *   row_loss = f * w * temperature^2 * sum_k p_k (ln p_k - ln q[id_k]),  loss = sum of row_loss,
+ *   grad_v   = f * w * temperature * (q_v - sum of p_k over the slots with id v) * up,    f = factor (/ *avg_factor)
+ * Rows without teacher mass or with row_weight 0 give zeros whatever z holds; an id >= vocab makes its row NaN.  top <= 256.
+ * row_weight, avg_factor, up (one number, or one a row), grad, row_loss, loss may be NULL.  skip_if_one: do nothing where *up is 1
+ * (grad holds the result for that already).  The workspace is needed with `loss`.                                     */
+size_t omnihd_topk_distill_workspace_bytes(long long rows, int vocab, int top, int z_type);
+int omnihd_topk_distill(const void* z, int z_type, long long z_stride, const void* t, int t_type, long long t_stride, const void* ids,
+                        int wide_ids, long long ids_stride, const float* row_weight, long long rows, int vocab, int top,
+                        float temperature, float factor, const float* avg_factor, const float* up, int up_per_row, int skip_if_one,
+                        void* grad, long long grad_stride, float* row_loss, float* loss, void* workspace, size_t workspace_bytes,
+                        void* stream);
+
 #ifdef __cplusplus
 }
 #endif

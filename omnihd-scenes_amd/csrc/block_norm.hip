@@ -1,0 +1,473 @@
+// Norms before and after a block of a residual stream, fused with the block's gate and the residual scale.
+//
+//   norm(v; w) = v * rsqrt(mean(v^2) + eps) * w
+//   join:  x' = r * x + gate * norm(y; post),  h = norm(x'; next)          (post, gate, next may each be absent)
+//   alone: h = norm(x; next)                                              (y == NULL)
+//
+// Backward, with nh = y * ry, xh = x' * rx (ry, rx kept from the forward, 8 bytes a row), a = dh * next:
+//   t  = dx' + rx * (a - xh * mean(a * xh)),      dx = r * t,             dnext = sum_rows dh * xh
+//   m  = t * gate * post,  dy = ry * (m - nh * mean(m * nh)),             dpost = sum_rows t * gate * nh,  dgate = sum t * nh * post
+// x' is computed again in fp32 from x and y (which have to be read anyway) and not read back: its stored form is rounded, and weight
+// gradients in fp32 would carry that rounding (1e-3 of them for bf16 rows).
+//
+// Bound by HBM: 4 rows of D forward, 6 backward, about 50 operations an element in all.  So each row is read once into registers
+// (8 elements a lane and step, TPR lanes a row, TPR chosen so that a lane holds 8 or 16 elements), its one or two sums go over the
+// lanes by DPP (over LDS beyond a wave), and the column sums of the weight gradients stay in registers over all rows that a block
+// walks; only their block sums go through memory ([blocks][2][D] fp32), joined in a fixed order by a second launch.
+// With a gate per channel (or per sample and channel) S = sum_rows t * nh serves both gradients: dgate = S * post, dpost = sum S * gate.
+#include "token_vec.h"
+
+namespace omnihd {
+namespace {
+using namespace tok;
+
+enum { kGateNone = 0, kGateRows = 1, kGateToken = 2, kGateFull = 3 };
+
+struct BlockArgs {
+  const void *x, *y, *post, *gate, *next;
+  const void *dxo, *dh;                  // backward: gradients of x' and h (either may be NULL)
+  void *xo, *ho, *gx, *gy, *ggate;
+  float *stats, *part;
+  long long rows, xs, ys, gs, dxos, dhs; // row strides in elements (outputs are dense)
+  long long per_gate, per_split;         // rows of one gate row, of one block
+  int splits, dim, post_type, gate_type, next_type, gate_kind;
+  float r, eps;
+};
+
+template <int TPR> constexpr int threads_of() { return TPR > 256 ? TPR : 256; }
+
+template <typename TA, typename TX, int TPR, int NV, bool ODD, bool HASY>
+__global__ __launch_bounds__(threads_of<TPR>()) void k_block_fwd(BlockArgs a) {
+  constexpr int TPB = threads_of<TPR>(), RPB = TPB / TPR;
+  __shared__ float red[32];
+  int turn = 0;
+  const int t = threadIdx.x % TPR, sub = threadIdx.x / TPR, D = a.dim;
+  const float inv_d = 1.f / (float)D;
+  const bool post = HASY && a.post, one_gate = a.gate_kind == kGateRows && a.per_gate >= a.rows;
+  float gp[NV][8], wn[NV][8];            // post (times the gate, where one serves all rows) and next
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const int c = (j * TPR + t) * 8, left = D - c;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) gp[j][k] = wn[j][k] = 1.f;
+    if (left <= 0) continue;
+    if (post) load8_any<ODD>(a.post, a.post_type, c, left, gp[j]);
+    if (a.next) load8_any<ODD>(a.next, a.next_type, c, left, wn[j]);
+    if (HASY && one_gate) {
+      float g[8];
+      load8_any<ODD>(a.gate, a.gate_type, c, left, g);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) gp[j][k] *= g[k];
+    }
+  }
+  for (long long base = (long long)blockIdx.x * RPB; base < a.rows; base += (long long)gridDim.x * RPB) {
+    const long long row = base + sub;
+    const bool act = row < a.rows;
+    float x[NV][8], y[NV][8], ry = 1.f, rx = 1.f;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int c = (j * TPR + t) * 8, left = D - c;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) x[j][k] = y[j][k] = 0.f;
+      if (!act || left <= 0) continue;
+      load8<ODD>(static_cast<const TX*>(a.x) + row * a.xs + c, left, x[j]);
+      if (HASY) load8<ODD>(static_cast<const TA*>(a.y) + row * a.ys + c, left, y[j]);
+    }
+    if (HASY) {
+      if (post) {
+        float s = 0.f;
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+#pragma unroll
+          for (int k = 0; k < 8; ++k) s = fmaf(y[j][k], y[j][k], s);
+        ry = __builtin_amdgcn_rsqf(fmaf(group<TPR>(s, Add(), red, turn), inv_d, a.eps));
+      }
+      float scalar = ry;
+      if (a.gate_kind == kGateToken && act) scalar *= load1_any(a.gate, a.gate_type, row);
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        const int c = (j * TPR + t) * 8, left = D - c;
+        if (!act || left <= 0) continue;
+        float g[8];
+        const bool own_gate = a.gate_kind == kGateFull || (a.gate_kind == kGateRows && !one_gate);
+        if (own_gate) load8_any<ODD>(a.gate, a.gate_type, a.gate_kind == kGateFull ? row * a.gs + c : (row / a.per_gate) * a.gs + c, left, g);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const float w = own_gate ? gp[j][k] * g[k] : gp[j][k];
+          x[j][k] = fmaf(y[j][k] * scalar, w, a.r * x[j][k]);
+        }
+        if (ODD) {                       // what the row does not have stays out of the sums
+#pragma unroll
+          for (int k = 0; k < 8; ++k) x[j][k] = k < left ? x[j][k] : 0.f;
+        }
+        if (a.xo) store8<ODD>(static_cast<TX*>(a.xo) + row * D + c, left, x[j]);
+      }
+    }
+    if (a.next) {
+      float s = 0.f;
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int k = 0; k < 8; ++k) s = fmaf(x[j][k], x[j][k], s);
+      rx = __builtin_amdgcn_rsqf(fmaf(group<TPR>(s, Add(), red, turn), inv_d, a.eps));
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        const int c = (j * TPR + t) * 8, left = D - c;
+        if (!act || left <= 0) continue;
+        float h[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) h[k] = x[j][k] * rx * wn[j][k];
+        store8<ODD>(static_cast<TA*>(a.ho) + row * D + c, left, h);
+      }
+    }
+    if (a.stats && act && t == 0) *reinterpret_cast<float2*>(a.stats + 2 * row) = make_float2(ry, rx);
+  }
+}
+
+// One block: `per_split` rows of one gate row (blockIdx = gate row * splits + split).
+template <typename TA, typename TX, int TPR, int NV, bool ODD, bool HASY>
+__global__ __launch_bounds__(threads_of<TPR>()) void k_block_bwd(BlockArgs a) {
+  constexpr int TPB = threads_of<TPR>(), RPB = TPB / TPR;
+  __shared__ float red[32];
+  __shared__ float fold[RPB > 1 ? TPB * NV * 8 : 1];
+  int turn = 0;
+  const int t = threadIdx.x % TPR, sub = threadIdx.x / TPR, D = a.dim;
+  const float inv_d = 1.f / (float)D;
+  const bool post = HASY && a.post;
+  const long long grp = blockIdx.x / a.splits, first = grp * a.per_gate, lo = first + (blockIdx.x % a.splits) * a.per_split;
+  long long hi = lo + a.per_split;
+  if (hi > first + a.per_gate) hi = first + a.per_gate;
+  if (hi > a.rows) hi = a.rows;
+  float gp[NV][8], wn[NV][8], aw[NV][8], au[NV][8];
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const int c = (j * TPR + t) * 8, left = D - c;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) gp[j][k] = wn[j][k] = 1.f, aw[j][k] = au[j][k] = 0.f;
+    if (left <= 0) continue;
+    if (post) load8_any<ODD>(a.post, a.post_type, c, left, gp[j]);
+    if (a.next) load8_any<ODD>(a.next, a.next_type, c, left, wn[j]);
+    if (HASY && a.gate_kind == kGateRows) {
+      float g[8];
+      load8_any<ODD>(a.gate, a.gate_type, grp * a.gs + c, left, g);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) gp[j][k] *= g[k];
+    }
+  }
+  for (long long base = lo; base < hi; base += RPB) {
+    const long long row = base + sub;
+    const bool act = row < hi;
+    float x[NV][8], y[NV][8], d[NV][8], ry = 1.f, rx = 1.f, tok = 1.f;
+    if (act) {
+      const float2 s = *reinterpret_cast<const float2*>(a.stats + 2 * row);
+      ry = s.x; rx = s.y;
+      if (HASY && a.gate_kind == kGateToken) tok = load1_any(a.gate, a.gate_type, row);
+    }
+    float h[NV][8];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int c = (j * TPR + t) * 8, left = D - c;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) x[j][k] = y[j][k] = d[j][k] = h[j][k] = 0.f;
+      if (!act || left <= 0) continue;
+      if (a.dh) load8<ODD>(static_cast<const TX*>(a.x) + row * a.xs + c, left, x[j]);
+      if (HASY) load8<ODD>(static_cast<const TA*>(a.y) + row * a.ys + c, left, y[j]);
+      if (a.dxo) load8<ODD>(static_cast<const TX*>(a.dxo) + row * a.dxos + c, left, d[j]);
+      if (a.dh) load8<ODD>(static_cast<const TA*>(a.dh) + row * a.dhs + c, left, h[j]);
+    }
+    // y := nh; x := xh; d := t
+    if (HASY) {
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int k = 0; k < 8; ++k) y[j][k] *= ry;
+    }
+    float full[NV][8];
+    if (HASY && a.gate_kind == kGateFull) {
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        const int c = (j * TPR + t) * 8, left = D - c;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) full[j][k] = 0.f;
+        if (act && left > 0) load8_any<ODD>(a.gate, a.gate_type, row * a.gs + c, left, full[j]);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int k = 0; k < 8; ++k) full[j][k] = tok;
+    }
+    if (a.dh) {
+      float s = 0.f;
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const float xn = HASY ? fmaf(y[j][k], gp[j][k] * full[j][k], a.r * x[j][k]) : x[j][k];
+          x[j][k] = xn * rx;
+          au[j][k] = fmaf(h[j][k], x[j][k], au[j][k]);
+          h[j][k] *= wn[j][k];
+          s = fmaf(h[j][k], x[j][k], s);
+        }
+      s = group<TPR>(s, Add(), red, turn) * inv_d;
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int k = 0; k < 8; ++k) d[j][k] = fmaf(rx, h[j][k] - x[j][k] * s, d[j][k]);
+    }
+    if (a.gx) {
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        const int c = (j * TPR + t) * 8, left = D - c;
+        if (!act || left <= 0) continue;
+        float o[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) o[k] = (HASY ? a.r : 1.f) * d[j][k];
+        store8<ODD>(static_cast<TX*>(a.gx) + row * D + c, left, o);
+      }
+    }
+    if (!HASY) continue;
+    float s = 0.f;                       // sum of t * nh * post (* gate, unless the gate is the token's): mean(m * nh), a token gate's gradient
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int c = (j * TPR + t) * 8, left = D - c;
+      float dg[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const float tn = d[j][k] * y[j][k];
+        aw[j][k] = a.gate_kind == kGateRows ? aw[j][k] + tn : fmaf(tn, full[j][k], aw[j][k]);
+        dg[k] = tn * gp[j][k];
+        s = fmaf(dg[k], a.gate_kind == kGateFull ? full[j][k] : 1.f, s);
+        d[j][k] *= gp[j][k] * full[j][k];           // m
+      }
+      if (a.gate_kind == kGateFull && a.ggate && act && left > 0) store8_any<ODD>(a.ggate, a.gate_type, row * D + c, left, dg);
+    }
+    float mean = 0.f;
+    if (post || (a.gate_kind == kGateToken && a.ggate)) {
+      s = group<TPR>(s, Add(), red, turn);
+      if (a.gate_kind == kGateToken && a.ggate && act && t == 0) store1_any(a.ggate, a.gate_type, row, s);
+      if (post) mean = s * tok * inv_d;
+    }
+    if (a.gy) {
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        const int c = (j * TPR + t) * 8, left = D - c;
+        if (!act || left <= 0) continue;
+        float o[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) o[k] = ry * (d[j][k] - y[j][k] * mean);
+        store8<ODD>(static_cast<TA*>(a.gy) + row * D + c, left, o);
+      }
+    }
+  }
+  if (!a.part) return;
+#pragma unroll
+  for (int which = 0; which < 2; ++which) {
+    if (which == 0 && !HASY) continue;
+    if (which == 1 && !a.next) continue;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int c = (j * TPR + t) * 8, left = D - c;
+      float v[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = which ? au[j][k] : aw[j][k];
+      if constexpr (RPB > 1) {           // the block's rows side by side: added in the order of their places
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < 8; ++k) fold[k * TPB + threadIdx.x] = v[k];
+        __syncthreads();
+        if (sub == 0) {
+          for (int o = 1; o < RPB; ++o)
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] += fold[k * TPB + o * TPR + t];
+        }
+      }
+      if (sub == 0 && left > 0) store8<ODD>(a.part + ((long long)blockIdx.x * 2 + which) * D + c, left, v);
+    }
+  }
+}
+
+// Block sums -> dnext, dpost (tile 0 of the gates) and the gradient of each gate row.  32 columns by 32 places of the blocks.
+__global__ __launch_bounds__(1024) void k_block_cols(const float* __restrict__ part, int blocks, int splits, int dim, const void* post,
+                                                     int post_type, const void* gate, int gate_type, long long gs, int gate_kind,
+                                                     void* gpost, void* ggate, void* gnext, int next_type) {
+  __shared__ float s0[32][33], s1[32][33];
+  const int tiles = (dim + 31) / 32, c = (blockIdx.x % tiles) * 32 + (threadIdx.x & 31), place = threadIdx.x >> 5;
+  const long long grp = (long long)(blockIdx.x / tiles) - 1;
+  float w = 0.f, u = 0.f;
+  if (c < dim) {
+    if (grp < 0) {
+      for (int b = place; b < blocks; b += 32) {
+        if (gpost) {
+          const float v = part[(long long)b * 2 * dim + c];
+          w += gate_kind == kGateRows ? v * load1_any(gate, gate_type, (long long)(b / splits) * gs + c) : v;
+        }
+        if (gnext) u += part[((long long)b * 2 + 1) * dim + c];
+      }
+    } else {
+      for (int b = place; b < splits; b += 32) w += part[(grp * splits + b) * 2 * dim + c];
+    }
+  }
+  s0[place][threadIdx.x & 31] = w;
+  s1[place][threadIdx.x & 31] = u;
+  __syncthreads();
+  if (place == 0 && c < dim) {
+    for (int o = 1; o < 32; ++o) w += s0[o][threadIdx.x], u += s1[o][threadIdx.x];
+    if (grp >= 0) store1_any(ggate, gate_type, grp * dim + c, post ? w * load1_any(post, post_type, c) : w);
+    else {
+      if (gpost) store1_any(gpost, post_type, c, w);
+      if (gnext) store1_any(gnext, next_type, c, u);
+    }
+  }
+}
+
+constexpr int kMaxDim = 16384;
+
+// lanes of a row: 8 elements a lane up to 512 columns, 16 beyond
+int lanes_of(int dim) {
+  if (dim <= 64) return 8;
+  if (dim <= 128) return 16;
+  if (dim <= 256) return 32;
+  if (dim <= 1024) return 64;
+  if (dim <= 2048) return 128;
+  if (dim <= 4096) return 256;
+  return dim <= 8192 ? 512 : 1024;
+}
+
+// Rows of one gate row are cut into as many blocks as fill the card three times over (a backward block of 256 threads needs about
+// 160 registers: three fit a CU), but no block gets fewer rows than it has places for.
+void split_of(long long rows, int dim, int gate_kind, long long per_gate, long long* groups, int* splits, long long* per_split) {
+  const long long per = gate_kind == kGateRows ? per_gate : rows;
+  *groups = rows > 0 ? (rows + per - 1) / per : 0;
+  const int tpr = lanes_of(dim), tpb = tpr > 256 ? tpr : 256, rpb = tpb / tpr, want = 3 * kCUs * 256 / tpb;
+  long long s = (want + *groups - 1) / (*groups > 0 ? *groups : 1), most = (per + rpb - 1) / rpb;
+  if (s > most) s = most;
+  if (s < 1) s = 1;
+  *per_split = ((per + s - 1) / s + rpb - 1) / rpb * rpb;
+  *splits = per > 0 ? (int)((per + *per_split - 1) / *per_split) : 1;
+}
+
+template <typename TA, typename TX, int TPR, int NV, bool ODD, bool HASY>
+void launch(const BlockArgs& a, bool bwd, long long blocks, hipStream_t st) {
+  constexpr int TPB = threads_of<TPR>(), RPB = TPB / TPR;
+  if (bwd) {
+    hipLaunchKernelGGL((k_block_bwd<TA, TX, TPR, NV, ODD, HASY>), dim3((unsigned)blocks), dim3(TPB), 0, st, a);
+  } else {
+    long long g = (a.rows + RPB - 1) / RPB, most = (long long)kMaxBlocks * 256 / TPB;
+    hipLaunchKernelGGL((k_block_fwd<TA, TX, TPR, NV, ODD, HASY>), dim3((unsigned)(g < most ? g : most)), dim3(TPB), 0, st, a);
+  }
+}
+template <typename TA, typename TX, bool ODD, bool HASY>
+void launch_dim(const BlockArgs& a, bool bwd, long long blocks, hipStream_t st) {
+  switch (lanes_of(a.dim)) {
+    case 8: return launch<TA, TX, 8, 1, ODD, HASY>(a, bwd, blocks, st);
+    case 16: return launch<TA, TX, 16, 1, ODD, HASY>(a, bwd, blocks, st);
+    case 32: return launch<TA, TX, 32, 1, ODD, HASY>(a, bwd, blocks, st);
+    case 64: return a.dim <= 512 ? launch<TA, TX, 64, 1, ODD, HASY>(a, bwd, blocks, st) : launch<TA, TX, 64, 2, ODD, HASY>(a, bwd, blocks, st);
+    case 128: return launch<TA, TX, 128, 2, ODD, HASY>(a, bwd, blocks, st);
+    case 256: return launch<TA, TX, 256, 2, ODD, HASY>(a, bwd, blocks, st);
+    case 512: return launch<TA, TX, 512, 2, ODD, HASY>(a, bwd, blocks, st);
+    default: return launch<TA, TX, 1024, 2, ODD, HASY>(a, bwd, blocks, st);
+  }
+}
+template <typename TA, typename TX>
+void launch_types(const BlockArgs& a, bool odd, bool bwd, long long blocks, hipStream_t st) {
+  if (a.y) return odd ? launch_dim<TA, TX, true, true>(a, bwd, blocks, st) : launch_dim<TA, TX, false, true>(a, bwd, blocks, st);
+  return odd ? launch_dim<TA, TX, true, false>(a, bwd, blocks, st) : launch_dim<TA, TX, false, false>(a, bwd, blocks, st);
+}
+
+bool vec_ok(const void* p, long long stride, int type) {
+  return !p || ((reinterpret_cast<uintptr_t>(p) & 15u) == 0 && (stride * type_size(type)) % 16 == 0);
+}
+
+int run_block(const BlockArgs& a, int x_type, int act_type, bool bwd, long long blocks, hipStream_t st) {
+  const int D = a.dim;
+  const bool vec = D % 8 == 0 && vec_ok(a.x, a.xs, x_type) && vec_ok(a.y, a.ys, act_type) && vec_ok(a.post, 0, 0) && vec_ok(a.next, 0, 0) &&
+                   (a.gate_kind == kGateToken || vec_ok(a.gate, a.gs, a.gate_type)) && vec_ok(a.dxo, a.dxos, x_type) &&
+                   vec_ok(a.dh, a.dhs, act_type) && vec_ok(a.xo, D, x_type) && vec_ok(a.ho, D, act_type) && vec_ok(a.gx, D, x_type) &&
+                   vec_ok(a.gy, D, act_type) && (a.gate_kind != kGateFull || vec_ok(a.ggate, D, a.gate_type)) && vec_ok(a.part, D, kF32);
+  if (act_type == kF32) launch_types<float, float>(a, !vec, bwd, blocks, st);
+  else if (act_type == kBF16 && x_type == kBF16) launch_types<__bf16, __bf16>(a, !vec, bwd, blocks, st);
+  else if (act_type == kBF16) launch_types<__bf16, float>(a, !vec, bwd, blocks, st);
+  else if (x_type == kF16) launch_types<_Float16, _Float16>(a, !vec, bwd, blocks, st);
+  else launch_types<_Float16, float>(a, !vec, bwd, blocks, st);
+  return check_launch(bwd ? "block_join_bwd" : "block_join_fwd");
+}
+
+}  // namespace
+}  // namespace omnihd
+
+using namespace omnihd;
+
+#define OMNIHD_BLOCK_CHECKS                                                                                                             \
+  OMNIHD_REQUIRE(rows >= 0 && rows < (1ll << 31) && dim >= 1 && dim <= kMaxDim, "0 <= rows < 2^31, 1 <= dim <= 16384");                  \
+  OMNIHD_REQUIRE(type_ok(x_type) && type_ok(act_type) && (x_type == act_type || x_type == kF32), "types: the stream has the block's type or fp32"); \
+  OMNIHD_REQUIRE((!post || type_ok(post_type)) && (!next || type_ok(next_type)) && (!gate || type_ok(gate_type)), "weight types");       \
+  OMNIHD_REQUIRE(gate_kind >= kGateNone && gate_kind <= kGateFull && (gate != nullptr) == (gate_kind != kGateNone), "gate and its kind"); \
+  OMNIHD_REQUIRE(gate_kind != kGateRows || rows_per_gate >= 1, "rows per gate");                                                        \
+  OMNIHD_REQUIRE(y || (!post && !gate && next), "without a block's output there is the next norm alone")
+
+extern "C" int omnihd_block_join_fwd(const void* x, long long x_stride, int x_type, const void* y, long long y_stride, int act_type,
+                                     const void* post, int post_type, const void* gate, int gate_type, int gate_kind,
+                                     long long gate_stride, long long rows_per_gate, const void* next, int next_type,
+                                     float residual_scale, float eps, long long rows, int dim, void* x_out, void* h_out, float* stats,
+                                     void* stream) {
+  OMNIHD_BLOCK_CHECKS;
+  if (rows == 0) return OMNIHD_OK;
+  OMNIHD_REQUIRE(x && (!y || x_out) && (!next || h_out), "null pointer");
+  BlockArgs a{};
+  a.x = x; a.y = y; a.post = post; a.gate = gate; a.next = next; a.xo = y ? x_out : nullptr; a.ho = h_out; a.stats = stats;
+  a.rows = rows; a.xs = x_stride; a.ys = y_stride; a.gs = gate_stride; a.per_gate = rows_per_gate;
+  a.dim = dim; a.post_type = post_type; a.gate_type = gate_type; a.next_type = next_type; a.gate_kind = gate_kind;
+  a.r = residual_scale; a.eps = eps;
+  return run_block(a, x_type, act_type, false, 0, (hipStream_t)stream);
+}
+
+extern "C" size_t omnihd_block_join_bwd_workspace_bytes(long long rows, int dim, int gate_kind, long long rows_per_gate) {
+  if (rows <= 0 || dim < 1 || (gate_kind == kGateRows && rows_per_gate < 1)) return 256;
+  long long groups, per_split;
+  int splits;
+  split_of(rows, dim, gate_kind, rows_per_gate, &groups, &splits, &per_split);
+  return (size_t)groups * splits * 2 * dim * sizeof(float);
+}
+
+extern "C" int omnihd_block_join_bwd(const void* x, long long x_stride, int x_type, const void* y, long long y_stride, int act_type,
+                                     const void* post, int post_type, const void* gate, int gate_type, int gate_kind,
+                                     long long gate_stride, long long rows_per_gate, const void* next, int next_type,
+                                     float residual_scale, long long rows, int dim, const float* stats, const void* dx_out,
+                                     long long dx_out_stride, const void* dh, long long dh_stride, void* gx, void* gy, void* g_post,
+                                     void* g_gate, void* g_next, void* workspace, size_t workspace_bytes, void* stream) {
+  OMNIHD_BLOCK_CHECKS;
+  OMNIHD_REQUIRE((g_post == nullptr || post) && (g_gate == nullptr || gate) && (g_next == nullptr || next), "a gradient without its input");
+  OMNIHD_REQUIRE((gy == nullptr || y) && (dh == nullptr || next), "a gradient without its input");
+  hipStream_t st = (hipStream_t)stream;
+  long long groups = 0, per_split = 1;
+  int splits = 1;
+  split_of(rows, dim, gate_kind, rows_per_gate, &groups, &splits, &per_split);
+  const long long blocks = groups * splits, tiles = (dim + 31) / 32;
+  const bool rows_gate = gate_kind == kGateRows && g_gate;
+  const bool cols = g_post || g_next || rows_gate;
+  OMNIHD_REQUIRE(blocks < (1ll << 31) && tiles * (1 + groups) < (1ll << 31), "grid");
+  if (rows > 0) {
+    OMNIHD_REQUIRE(x && stats, "null pointer");
+    if (cols) {
+      OMNIHD_REQUIRE(workspace, "null pointer");
+      const size_t need = (size_t)blocks * 2 * dim * sizeof(float);
+      if (workspace_bytes < need) { set_error("block_join_bwd: workspace %zu < required %zu", workspace_bytes, need); return OMNIHD_ERR_WORKSPACE; }
+    }
+    BlockArgs a{};
+    a.x = x; a.y = y; a.post = post; a.gate = gate; a.next = next; a.dxo = dx_out; a.dh = dh; a.gx = gx; a.gy = gy;
+    a.ggate = gate_kind == kGateRows ? nullptr : g_gate; a.stats = const_cast<float*>(stats);
+    a.part = cols ? static_cast<float*>(workspace) : nullptr;
+    a.rows = rows; a.xs = x_stride; a.ys = y_stride; a.gs = gate_stride; a.dxos = dx_out_stride; a.dhs = dh_stride;
+    a.per_gate = gate_kind == kGateRows ? rows_per_gate : rows; a.per_split = per_split; a.splits = splits;
+    a.dim = dim; a.post_type = post_type; a.gate_type = gate_type; a.next_type = next_type; a.gate_kind = gate_kind; a.r = residual_scale;
+    const int rc = run_block(a, x_type, act_type, true, blocks, st);
+    if (rc != OMNIHD_OK) return rc;
+  }
+  if (cols)                              // with no rows the weights' gradients are zero: no block, no gate row
+    hipLaunchKernelGGL(k_block_cols, dim3((unsigned)(tiles * (1 + (rows_gate ? groups : 0)))), dim3(1024), 0, st,
+                       static_cast<const float*>(workspace), (int)blocks, splits, dim, post, post_type, gate, gate_type, gate_stride,
+                       gate_kind, g_post, g_gate, g_next, next_type);
+  return check_launch("block_join_bwd");
+}

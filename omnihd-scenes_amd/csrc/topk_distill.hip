@@ -1,0 +1,473 @@
+// Distillation from a teacher's top logits: the loss and its gradient in one pass over the student's logits.
+//
+//   p = softmax over the filled slots of t_k / T          (K slots a row, id < 0: an empty slot)
+//   q = softmax(z / T) over the V entries of the row
+//   row  = T^2 * sum_k p_k (ln p_k - ln q[id_k])          loss = factor * sum_rows w * row      (or factor * w * row, row by row)
+//   dz_v = factor * w * T * (q_v - sum_{k: id_k = v} p_k) (* up: the gradient that arrives at the loss)
+//
+// A row with no teacher mass (no filled slot, or all of them -inf) or of weight 0 adds exactly 0 and gets a zero gradient, whatever
+// its logits hold; an id >= V makes its row NaN (nothing outside the row is read or written).
+//
+// Bound by HBM at large V: V read, V written; about 15 operations an element (two exponentials among them) take half as long.  So a row
+// is read once into registers (16 bytes a lane and step), its maximum and its sum of exponentials go over the lanes that share it, and the
+// gradient is written from the registers.  Rows beyond 64 K (16-bit) entries are read twice, the second time out of the caches.  All in base 2:
+// exp2(z * c - m * c), c = log2(e) / T, one fused multiply-add with a single rounding of the difference; sums in fp32.
+// The few entries that the teacher names are written again behind the row's own stores, from their own p sums (slots with the same id are
+// summed by the first of them, so an id may stand in a row more than once).
+// Rows of up to 32 entries (the classes of a detection or occupancy head) take a lane each.
+#include "token_vec.h"
+
+namespace omnihd {
+namespace {
+using namespace tok;
+
+constexpr int kMaxTop = 256;
+constexpr float kLn2 = 0.69314718055994531f;
+
+struct DistillArgs {
+  const void *z, *t, *ids;
+  const float *w, *up, *avg;             // row weights, gradient of the loss (up_step 0: one for all rows), divisor on the device: each may be NULL
+  void* g;                               // gradient of z (NULL: not asked for)
+  float *rows_out, *sums;                // per-row losses, or one sum a block; both may be NULL
+  long long rows, zs, gs, ts, is;        // rows and row strides in elements
+  int vocab, top, t_type, wide_ids, up_step, skip_if_one;
+  float temperature, factor;
+};
+
+__device__ __forceinline__ long long id_at(const DistillArgs& a, long long at) {
+  return a.wide_ids ? static_cast<const long long*>(a.ids)[at] : (long long)static_cast<const int*>(a.ids)[at];
+}
+__device__ __forceinline__ float factor_of(const DistillArgs& a) { return a.avg ? a.factor / *a.avg : a.factor; }
+
+// 16 bytes of logits, kept as they are
+template <typename T> struct Pack { static constexpr int n = 16 / (int)sizeof(T); typedef T V __attribute__((ext_vector_type(16 / sizeof(T)))); };
+template <bool ODD, typename T>
+__device__ __forceinline__ typename Pack<T>::V load_pack(const T* __restrict__ p, int left) {
+  typedef typename Pack<T>::V V;
+  typedef V W __attribute__((aligned(ODD ? sizeof(T) : 16)));
+  if (!ODD || left >= Pack<T>::n) return *reinterpret_cast<const W*>(p);
+  V v;
+#pragma unroll
+  for (int k = 0; k < Pack<T>::n; ++k) v[k] = k < left ? p[k] : (T)-__builtin_inff();
+  return v;
+}
+template <bool ODD, typename T>
+__device__ __forceinline__ void store_pack(T* __restrict__ p, int left, const typename Pack<T>::V& v) {
+  typedef typename Pack<T>::V V;
+  typedef V W __attribute__((aligned(ODD ? sizeof(T) : 16)));
+  if (!ODD || left >= Pack<T>::n) { *reinterpret_cast<W*>(p) = v; return; }
+#pragma unroll
+  for (int k = 0; k < Pack<T>::n; ++k)
+    if (k < left) p[k] = v[k];
+}
+
+// NaN where either is NaN (fmaxf drops it: a NaN logit has to reach the loss)
+struct MaxNan { __device__ __forceinline__ float operator()(float a, float b) const { return (a != a || b != b) ? __builtin_nanf("") : fmaxf(a, b); } };
+
+// a product as it was rounded: the compiler may not take it into a fused multiply-add
+__device__ __forceinline__ float rounded(float v) { asm volatile("" : "+v"(v)); return v; }
+
+// TPR lanes a row; NV steps of 16 bytes a lane in registers, or (NV = 0) the row is read twice.
+template <typename T, int TPR, int NV, bool ODD>
+__global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_distill_rows(DistillArgs a) {
+  constexpr int TPB = TPR > 256 ? TPR : 256, RPB = TPB / TPR, VE = Pack<T>::n, SL = TPR < 64 ? TPR : 64, KEEP = NV ? NV : 1;
+  typedef typename Pack<T>::V V;
+  __shared__ float red[32], row_coef[RPB], row_sum[RPB];
+  extern __shared__ float slots[];       // [RPB][2][K]: ids and teacher values
+  if (a.skip_if_one && *a.up == 1.f) return;
+  int turn = 0;
+  const int t = threadIdx.x % TPR, sub = threadIdx.x / TPR, K = a.top;
+  int* sid = reinterpret_cast<int*>(slots) + sub * 2 * K;
+  float* st = slots + sub * 2 * K + K;
+  const float c = 1.44269504088896341f / a.temperature, base = factor_of(a);
+  float total = 0.f;
+  for (long long first = (long long)blockIdx.x * RPB; first < a.rows; first += (long long)gridDim.x * RPB) {
+    const long long row = first + sub;
+    const bool act = row < a.rows;
+    const T* z = static_cast<const T*>(a.z) + (act ? row : 0) * a.zs;
+    const float w = !act ? 0.f : a.w ? a.w[row] : 1.f;
+    // the teacher: lanes t < SL of the row's first wave
+    float coef = 0.f, mt = -__builtin_inff(), ls = 0.f;
+    if (TPR <= 64 || t < 64) {
+      bool bad = false;
+      if (w != 0.f)
+        for (int k = t; k < K; k += SL) {
+          const long long id = id_at(a, row * a.is + k);
+          const float v = id < 0 ? -__builtin_inff() : load1_any(a.t, a.t_type, row * a.ts + k);
+          bad |= id >= a.vocab;
+          sid[k] = id < 0 || id >= a.vocab ? -1 : (int)id;
+          st[k] = v;
+          mt = MaxNan()(mt, v);
+        }
+      mt = lanes<SL>(mt, MaxNan());
+      bad = (bool)lanes<SL>(bad ? 1.f : 0.f, Max());
+      const bool some = w != 0.f && mt != -__builtin_inff();
+      const float mtc = rounded(mt * c);
+      float s = 0.f;
+      if (some)
+        for (int k = t; k < K; k += SL) {
+          const float d = fmaf(st[k], c, -mtc);
+          st[k] = d;                               // log2 of p, short of the sum's
+          s += __builtin_amdgcn_exp2f(d);
+        }
+      s = lanes<SL>(s, Add());
+      ls = some ? __builtin_amdgcn_logf(s) : 0.f;        // base 2
+      coef = some ? w : 0.f;
+      if (bad) coef = __builtin_nanf("");
+      if (TPR > 64 && t == 0) row_coef[sub] = coef;
+    }
+    // the row's maximum and sum
+    V keep[KEEP];
+    float m = -__builtin_inff(), s = 0.f, own_mc = 0.f;
+    if (w != 0.f) {
+      if constexpr (NV > 0) {
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+          const int at = (j * TPR + t) * VE, left = a.vocab - at;
+          if (left > 0) keep[j] = load_pack<ODD>(z + at, left);
+        }
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+          if ((j * TPR + t) * VE < a.vocab)
+#pragma unroll
+            for (int k = 0; k < VE; ++k) m = fmaxf(m, (float)keep[j][k]);
+      } else {
+        for (int at = t * VE; at < a.vocab; at += TPR * VE) {
+          const V v = load_pack<ODD>(z + at, a.vocab - at);
+          float big = (float)v[0];
+#pragma unroll
+          for (int k = 1; k < VE; ++k) big = fmaxf(big, (float)v[k]);
+          if (big > m) {                           // (rescaled by the difference of the ROUNDED products that the terms are shifted by)
+            const float to = rounded(big * c);
+            s = m == -__builtin_inff() ? s : s * __builtin_amdgcn_exp2f(own_mc - to);
+            m = big;
+            own_mc = to;
+          }
+#pragma unroll
+          for (int k = 0; k < VE; ++k) s += __builtin_amdgcn_exp2f(fmaf((float)v[k], c, -own_mc));
+        }
+      }
+    }
+    const float own = m;
+    m = group<TPR>(m, Max(), red, turn);
+    const float mc = rounded(m * c);
+    if (w != 0.f) {
+      if constexpr (NV > 0) {
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+          if ((j * TPR + t) * VE < a.vocab)
+#pragma unroll
+            for (int k = 0; k < VE; ++k) s += __builtin_amdgcn_exp2f(fmaf((float)keep[j][k], c, -mc));
+      } else if (own == -__builtin_inff()) {
+        if (m == own && t * VE < a.vocab) s = __builtin_nanf("");   // nothing but -inf in the row
+      } else {
+        s *= __builtin_amdgcn_exp2f(own_mc - mc);
+      }
+    }
+    s = group<TPR>(s, Add(), red, turn);
+    if (TPR > 64) coef = row_coef[sub];            // behind the barriers of the sums
+    const float scale = base * coef * a.temperature;
+    float up = 1.f;
+    if (a.up) up = act ? a.up[a.up_step ? row : 0] : 0.f;
+    const float k1 = coef == 0.f ? 0.f : scale * up, kq = k1 / s;
+    if (a.g && act) {
+      T* g = static_cast<T*>(a.g) + row * a.gs;
+      if (k1 == 0.f) {                             // nothing to learn from this row
+        V zero;
+#pragma unroll
+        for (int k = 0; k < VE; ++k) zero[k] = (T)0.f;
+        for (int at = t * VE; at < a.vocab; at += TPR * VE) store_pack<ODD>(g + at, a.vocab - at, zero);
+      } else if constexpr (NV > 0) {
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+          const int at = (j * TPR + t) * VE, left = a.vocab - at;
+          if (left <= 0) continue;
+          V o;
+#pragma unroll
+          for (int k = 0; k < VE; ++k) o[k] = (T)(__builtin_amdgcn_exp2f(fmaf((float)keep[j][k], c, -mc)) * kq);
+          store_pack<ODD>(g + at, left, o);
+        }
+      } else {
+        for (int at = t * VE; at < a.vocab; at += TPR * VE) {
+          const V v = load_pack<ODD>(z + at, a.vocab - at);
+          V o;
+#pragma unroll
+          for (int k = 0; k < VE; ++k) o[k] = (T)(__builtin_amdgcn_exp2f(fmaf((float)v[k], c, -mc)) * kq);
+          store_pack<ODD>(g + at, a.vocab - at, o);
+        }
+      }
+    }
+    // the teacher's entries, behind the stores of the whole row
+    if (TPR > 64) __syncthreads();
+    else {
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+    }
+    if (TPR <= 64 || t < 64) {
+      float part = 0.f;
+      if (coef != 0.f && act) {
+        const float lq = __builtin_amdgcn_logf(s);
+        for (int k = t; k < K; k += SL) {
+          const int id = sid[k];
+          if (id < 0) continue;
+          const float lp = st[k] - ls, p = __builtin_amdgcn_exp2f(lp), zk = fmaf((float)z[id], c, -mc);
+          if (!(p == 0.f)) part = fmaf(p, lp - (zk - lq), part);
+          if (!a.g || k1 == 0.f) continue;
+          float sum = 0.f;                         // p of every slot with this id; only the first of them writes
+          bool leads = true;
+          for (int o = 0; o < K; ++o)
+            if (sid[o] == id) {
+              leads &= o >= k;
+              sum += __builtin_amdgcn_exp2f(st[o] - ls);
+            }
+          if (leads) static_cast<T*>(a.g)[row * a.gs + id] = (T)fmaf(__builtin_amdgcn_exp2f(zk), kq, -k1 * sum);
+        }
+      }
+      part = lanes<SL>(part, Add());
+      float loss = coef == 0.f ? 0.f : base * coef * a.temperature * a.temperature * kLn2 * part;
+      if (t == 0 && act) {
+        if (a.rows_out) a.rows_out[row] = loss;
+        total += loss;
+      }
+    }
+    if (TPR > 64) __syncthreads();                 // the slots are written again
+    else {
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+    }
+  }
+  if (a.sums) {
+    if (t == 0) row_sum[sub] = total;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      for (int o = 1; o < RPB; ++o) total += row_sum[o];
+      a.sums[blockIdx.x] = total;
+    }
+  }
+}
+
+// A lane a row, up to VM entries in registers; the first KR slots too.
+template <typename T, int VM>
+__global__ __launch_bounds__(256) void k_distill_lanes(DistillArgs a) {
+  constexpr int VE = Pack<T>::n, NP = VM / VE, KR = 8;
+  typedef typename Pack<T>::V V;
+  __shared__ float wave_sum[4];
+  if (a.skip_if_one && *a.up == 1.f) return;
+  const float c = 1.44269504088896341f / a.temperature, base = factor_of(a);
+  float total = 0.f;
+  for (long long row = (long long)blockIdx.x * 256 + threadIdx.x; row < a.rows; row += (long long)gridDim.x * 256) {
+    const float w = a.w ? a.w[row] : 1.f;
+    const T* z = static_cast<const T*>(a.z) + row * a.zs;
+    const int K = a.top, V_ = a.vocab;
+    float x[VM], m = -__builtin_inff(), s = 0.f;
+    int id[KR];
+    float tv[KR], mt = -__builtin_inff();
+    bool bad = false;
+#pragma unroll
+    for (int j = 0; j < NP; ++j) {
+      if (j * VE < V_) {
+        const V v = load_pack<true>(z + j * VE, V_ - j * VE);
+#pragma unroll
+        for (int k = 0; k < VE; ++k) x[j * VE + k] = (float)v[k];
+      } else {
+#pragma unroll
+        for (int k = 0; k < VE; ++k) x[j * VE + k] = -__builtin_inff();
+      }
+    }
+    auto slot = [&](int k, int& i, float& v) {
+      const long long full = id_at(a, row * a.is + k);
+      v = full < 0 ? -__builtin_inff() : load1_any(a.t, a.t_type, row * a.ts + k);
+      bad |= full >= V_;
+      i = full < 0 || full >= V_ ? -1 : (int)full;
+    };
+#pragma unroll
+    for (int k = 0; k < KR; ++k) {
+      id[k] = -1; tv[k] = -__builtin_inff();
+      if (k < K) { slot(k, id[k], tv[k]); mt = MaxNan()(mt, tv[k]); }
+    }
+    for (int k = KR; k < K; ++k) {
+      int i; float v;
+      slot(k, i, v);
+      mt = MaxNan()(mt, v);
+    }
+#pragma unroll
+    for (int k = 0; k < VM; ++k) m = fmaxf(m, x[k]);
+    const float mc = rounded(m * c);
+#pragma unroll
+    for (int k = 0; k < VM; ++k) {
+      if (k < V_) { x[k] = fmaf(x[k], c, -mc); s += __builtin_amdgcn_exp2f(x[k]); }
+    }
+    const bool some = mt != -__builtin_inff();
+    const float mtc = rounded(mt * c);
+    float sum = 0.f;
+#pragma unroll
+    for (int k = 0; k < KR; ++k) if (k < K) sum += __builtin_amdgcn_exp2f(fmaf(tv[k], c, -mtc));
+    for (int k = KR; k < K; ++k) {
+      int i; float v;
+      slot(k, i, v);
+      sum += __builtin_amdgcn_exp2f(fmaf(v, c, -mtc));
+    }
+    float coef = w != 0.f && some ? w : 0.f;
+    if (bad && w != 0.f) coef = __builtin_nanf("");
+    const float ls = __builtin_amdgcn_logf(sum), lq = __builtin_amdgcn_logf(s);
+    float up = 1.f;
+    if (a.up) up = a.up[a.up_step ? row : 0];
+    const float k1 = coef == 0.f ? 0.f : base * coef * a.temperature * up, kq = k1 / s;
+    float mass[VM], part = 0.f;
+#pragma unroll
+    for (int k = 0; k < VM; ++k) mass[k] = 0.f;
+    auto use = [&](int i, float v) {
+      if (i < 0) return;
+      const float lp = fmaf(v, c, -mtc) - ls, p = __builtin_amdgcn_exp2f(lp);
+      float zk = 0.f;
+#pragma unroll
+      for (int q = 0; q < VM; ++q) {
+        mass[q] += q == i ? p : 0.f;
+        zk = q == i ? x[q] : zk;
+      }
+      if (!(p == 0.f)) part = fmaf(p, lp - (zk - lq), part);
+    };
+    if (coef != 0.f) {
+#pragma unroll
+      for (int k = 0; k < KR; ++k) if (k < K) use(id[k], tv[k]);
+      for (int k = KR; k < K; ++k) {
+        int i; float v;
+        slot(k, i, v);
+        use(i, v);
+      }
+    }
+    if (a.g) {
+      T* g = static_cast<T*>(a.g) + row * a.gs;
+#pragma unroll
+      for (int j = 0; j < NP; ++j) {
+        if (j * VE >= V_) continue;
+        V o;
+#pragma unroll
+        for (int k = 0; k < VE; ++k)
+          o[k] = (T)(k1 == 0.f ? 0.f : fmaf(__builtin_amdgcn_exp2f(x[j * VE + k]), kq, -k1 * mass[j * VE + k]));
+        store_pack<true>(g + j * VE, V_ - j * VE, o);
+      }
+    }
+    const float loss = coef == 0.f ? 0.f : base * coef * a.temperature * a.temperature * kLn2 * part;
+    if (a.rows_out) a.rows_out[row] = loss;
+    total += loss;
+  }
+  if (a.sums) {
+    total = lanes<64>(total, Add());
+    if ((threadIdx.x & 63) == 0) wave_sum[threadIdx.x >> 6] = total;
+    __syncthreads();
+    if (threadIdx.x == 0) a.sums[blockIdx.x] = (wave_sum[0] + wave_sum[1]) + (wave_sum[2] + wave_sum[3]);
+  }
+}
+
+__global__ __launch_bounds__(1024) void k_distill_total(const float* __restrict__ sums, int n, float* __restrict__ loss) {
+  __shared__ double wave_sum[16];
+  double s = 0;
+  for (int i = threadIdx.x; i < n; i += 1024) s += sums[i];
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) s += __shfl_xor(s, o, 64);
+  if ((threadIdx.x & 63) == 0) wave_sum[threadIdx.x >> 6] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int i = 1; i < 16; ++i) s += wave_sum[i];
+    *loss = (float)s;
+  }
+}
+
+struct Geometry { int tpr, nv; };       // nv 0: the row is read twice
+template <typename T> Geometry geometry(int vocab, int top) {
+  const long long packs = (vocab + Pack<T>::n - 1) / Pack<T>::n;
+  int tpr = 8;
+  while (tpr < 64 && (packs > tpr || (256 / tpr) * 8 * top > 32768)) tpr *= 2;
+  if (packs <= tpr) return {tpr, 1};
+  if (packs <= 64 * 4) return {64, 4};
+  if (packs <= 256 * 4) return {256, 4};
+  if (packs <= 256 * 8) return {256, 8};
+  if (packs <= 1024 * 4) return {1024, 4};
+  if (packs <= 1024 * 8) return {1024, 8};
+  return {1024, 0};
+}
+bool by_lanes(int vocab) { return vocab <= 32; }
+template <typename T> int blocks_of(long long rows, int vocab, int top) {
+  if (by_lanes(vocab)) return grid_for(rows, 256);
+  const int tpr = geometry<T>(vocab, top).tpr, tpb = tpr > 256 ? tpr : 256;
+  const long long g = (rows + tpb / tpr - 1) / (tpb / tpr), most = (long long)kMaxBlocks * 256 / tpb;
+  return (int)(g < most ? g : most);
+}
+int blocks_of_type(int type, long long rows, int vocab, int top) {
+  if (rows <= 0) return 1;
+  return type == kF32 ? blocks_of<float>(rows, vocab, top) : blocks_of<__bf16>(rows, vocab, top);
+}
+
+template <typename T, bool ODD>
+void launch_rows(const DistillArgs& a, int blocks, hipStream_t st) {
+  const Geometry g = geometry<T>(a.vocab, a.top);
+  const int tpb = g.tpr > 256 ? g.tpr : 256;
+  const size_t lds = (size_t)(tpb / g.tpr) * 2 * a.top * sizeof(float);
+#define OMNIHD_DISTILL(R, N) hipLaunchKernelGGL((k_distill_rows<T, R, N, ODD>), dim3(blocks), dim3(tpb), lds, st, a)
+  if (g.tpr == 8) OMNIHD_DISTILL(8, 1);
+  else if (g.tpr == 16) OMNIHD_DISTILL(16, 1);
+  else if (g.tpr == 32) OMNIHD_DISTILL(32, 1);
+  else if (g.tpr == 64 && g.nv == 1) OMNIHD_DISTILL(64, 1);
+  else if (g.tpr == 64) OMNIHD_DISTILL(64, 4);
+  else if (g.tpr == 256 && g.nv == 4) OMNIHD_DISTILL(256, 4);
+  else if (g.tpr == 256) OMNIHD_DISTILL(256, 8);
+  else if (g.nv == 4) OMNIHD_DISTILL(1024, 4);
+  else if (g.nv == 8) OMNIHD_DISTILL(1024, 8);
+  else OMNIHD_DISTILL(1024, 0);
+#undef OMNIHD_DISTILL
+}
+template <typename T>
+void launch_distill(const DistillArgs& a, int blocks, hipStream_t st) {
+  if (by_lanes(a.vocab)) {
+    if (a.vocab <= 16) hipLaunchKernelGGL((k_distill_lanes<T, 16>), dim3(blocks), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((k_distill_lanes<T, 32>), dim3(blocks), dim3(256), 0, st, a);
+    return;
+  }
+  auto fits = [&](const void* p, long long stride) { return !p || ((reinterpret_cast<uintptr_t>(p) & 15u) == 0 && stride % Pack<T>::n == 0); };
+  if (a.vocab % Pack<T>::n == 0 && fits(a.z, a.zs) && fits(a.g, a.gs)) launch_rows<T, false>(a, blocks, st);
+  else launch_rows<T, true>(a, blocks, st);
+}
+
+}  // namespace
+}  // namespace omnihd
+
+using namespace omnihd;
+
+extern "C" size_t omnihd_topk_distill_workspace_bytes(long long rows, int vocab, int top, int z_type) {
+  if (rows < 0 || vocab < 1 || top < 1 || top > kMaxTop || !type_ok(z_type)) return 0;
+  return align_up((size_t)blocks_of_type(z_type, rows, vocab, top) * sizeof(float), 256);
+}
+
+extern "C" int omnihd_topk_distill(const void* z, int z_type, long long z_stride, const void* t, int t_type, long long t_stride,
+                                   const void* ids, int wide_ids, long long ids_stride, const float* row_weight, long long rows, int vocab,
+                                   int top, float temperature, float factor, const float* avg_factor, const float* up, int up_per_row,
+                                   int skip_if_one, void* grad, long long grad_stride, float* row_loss, float* loss, void* workspace,
+                                   size_t workspace_bytes, void* stream) {
+  OMNIHD_REQUIRE(rows >= 0 && rows < (1ll << 31) && vocab >= 1 && top >= 1 && top <= kMaxTop, "0 <= rows < 2^31, vocab >= 1, 1 <= top <= 256");
+  OMNIHD_REQUIRE(type_ok(z_type) && type_ok(t_type), "types");
+  OMNIHD_REQUIRE(temperature > 0.f, "temperature > 0");
+  OMNIHD_REQUIRE(!skip_if_one || (up && !up_per_row && !loss && !row_loss), "skip_if_one goes with one gradient for all rows");
+  hipStream_t st = (hipStream_t)stream;
+  const int blocks = blocks_of_type(z_type, rows, vocab, top);
+  float* sums = nullptr;
+  if (loss) {
+    const size_t need = omnihd_topk_distill_workspace_bytes(rows, vocab, top, z_type);
+    OMNIHD_REQUIRE(workspace, "null pointer");
+    if (workspace_bytes < need) { set_error("topk_distill: workspace %zu < required %zu", workspace_bytes, need); return OMNIHD_ERR_WORKSPACE; }
+    sums = static_cast<float*>(workspace);
+  }
+  if (rows > 0) {
+    OMNIHD_REQUIRE(z && t && ids && z_stride >= vocab && t_stride >= top && ids_stride >= top && (!grad || grad_stride >= vocab), "null pointer or short rows");
+    DistillArgs a{};
+    a.z = z; a.t = t; a.ids = ids; a.w = row_weight; a.up = up; a.avg = avg_factor; a.g = grad; a.rows_out = row_loss; a.sums = sums;
+    a.rows = rows; a.zs = z_stride; a.gs = grad_stride; a.ts = t_stride; a.is = ids_stride;
+    a.vocab = vocab; a.top = top; a.t_type = t_type; a.wide_ids = wide_ids; a.up_step = up_per_row; a.skip_if_one = skip_if_one;
+    a.temperature = temperature; a.factor = factor;
+    if (z_type == kF32) launch_distill<float>(a, blocks, st);
+    else if (z_type == kBF16) launch_distill<__bf16>(a, blocks, st);
+    else launch_distill<_Float16>(a, blocks, st);
+  }
+  if (loss) hipLaunchKernelGGL(k_distill_total, dim3(1), dim3(1024), 0, st, sums, rows > 0 ? blocks : 0, loss);
+  return check_launch("topk_distill");
+}

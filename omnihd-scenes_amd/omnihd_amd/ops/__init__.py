@@ -9,13 +9,16 @@
   streams       Weight gradients on a side stream (plain and under DistributedDataParallel bucket views) and the live fast-path report.
   conv_fp32     The fp32 step's convolutions as autograd Functions: fp32-grade split form (_ConvSplit) and TF32-grade half form (_ConvF16).
   conv_bf16     The bf16 step's convolutions and transposed convolutions as autograd Functions, bias gradients by column sums.
-  norm          BatchNorm epilogues as autograd Functions: frozen (affine + residual + ReLU) and training mode (csrc/affine_act.hip, batch_norm.hip).
-  misc          Deformable-convolution sampling, rotated NMS, fused anchor targets + detection losses (csrc/dcn_sample.hip, nms_rotated.hip, anchor_loss.hip).
+  norm          BatchNorm epilogues as autograd Functions: frozen (affine + residual + ReLU) and training mode (csrc/affine_act.hip, batch_norm.hip);
+                norms before and after a block of token rows with its gate and residual scale (csrc/block_norm.hip).
+  misc          Deformable-convolution sampling, rotated NMS, fused anchor targets + detection losses, token embedding, distillation from a teacher's
+                top logits (csrc/dcn_sample.hip, nms_rotated.hip, anchor_loss.hip, token_embed.hip, topk_distill.hip).
 Every top-level name of every part is re-exported here, private ones included: `ops.X` is the public face (tests spy on and
 replace functions through it); state that code REBINDS lives in one part and is reached through that part."""
 from . import _core
 from ._core import (_ptr, _current_device, _raw_stream, _stream, _want, _same_device, _workspace, _NULL_CTX, _SIZE_CACHE, _on,
-    _WGRAD_WS, _wgrad_workspace, _want_cl, _pair_same, deterministic, FAST_PATHS, _CL, _rows_view, _f32c)
+    _WGRAD_WS, _wgrad_workspace, _want_cl, _pair_same, deterministic, FAST_PATHS, _CL, _rows_view, _f32c,
+    _TYPE_CODE, _want_rows, _rows2d, _pitch)
 from . import pool
 from .pool import (bev_pool_v2_forward, bev_pool_v2_backward, bev_pool_v2_forward_csr, _PREFETCH_STREAMS, prefetch,
     bev_pool_v2_forward_direct, bev_pool_v2_backward_patch, tile_descriptors, csr_tiles, _nhwc_rows, _DepthHead,
@@ -56,8 +59,10 @@ from .conv_bf16 import (_ConvBiasColsum, wgrad_split_padded, conv_bias_colsum_su
     conv3x3, conv_hip_wgrad, _gen_or_library, _deconv_as_conv, _DeconvHipWgrad, _DeconvSplit, deconv_split_supported,
     deconv_split, deconv_supported, deconv_hip_wgrad)
 from . import norm
-from .norm import (_AffineAct, affine_act_supported, affine_act, _BnTrainAct, bn_train_supported, bn_train_act)
+from .norm import (_AffineAct, affine_act_supported, affine_act, _BnTrainAct, bn_train_supported, bn_train_act, _BLOCK_MAX_DIM, _GATE_NONE, _GATE_ROWS,
+    _GATE_TOKEN, _GATE_FULL, _gate_layout, _block_args, _BlockJoin, _block_forward, _block_checks, block_norm, block_join)
 from . import misc
-from .misc import (_DcnSample, dcn3x3_sample, dcn3x3_supported, nms_rotated, iou_bev_matrix, _AnchorLoss, anchor_loss)
+from .misc import (_DcnSample, dcn3x3_sample, dcn3x3_supported, nms_rotated, iou_bev_matrix, _AnchorLoss, anchor_loss,
+    _embed_forward, _TokenEmbed, token_embedding, _DISTILL_MAX_TOP, _distill_call, _TopkDistill, topk_distill_loss)
 
 PARTS = (_core, pool, radar, conv_kernels, policy, planes, weights, streams, conv_fp32, conv_bf16, norm, misc)

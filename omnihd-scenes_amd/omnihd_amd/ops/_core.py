@@ -119,3 +119,34 @@ def _rows_view(t):
 def _f32c(t):
     # only the data pointer is read: a contiguous fp32 parameter is used as it is (no detach() object per call)
     return t if (t.dtype == torch.float32 and t.is_contiguous()) else t.detach().float().contiguous()
+
+
+# --------------------------------------------------------------------------------------------
+# Token rows (norms of a residual stream, embedding, distillation)
+# --------------------------------------------------------------------------------------------
+_TYPE_CODE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}       # include/omnihd_hip.h: element type codes
+
+
+def _want_rows(t, name):
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise RuntimeError(f"{name} must be a CUDA(HIP) tensor; the HIP ops have no CPU path")
+    if t.dtype not in _TYPE_CODE:
+        raise TypeError(f"{name} must be float32, bfloat16 or float16, got {t.dtype}")
+
+
+def _rows2d(t, dim):
+    """(..., dim) as rows with one pitch between them: a view where the strides allow it, else a copy."""
+    if t.is_contiguous():
+        return t.view(-1, dim)
+    if dim == 1 or t.stride(-1) == 1:
+        try:
+            v = t.view(-1, dim)
+        except RuntimeError:
+            v = None
+        if v is not None and (v.shape[0] <= 1 or v.stride(0) >= dim):
+            return v
+    return t.contiguous().view(-1, dim)
+
+
+def _pitch(rows):
+    return rows.stride(0) if rows.shape[0] > 1 else rows.shape[1]

@@ -1,16 +1,19 @@
-"""Deformable-convolution sampling, rotated NMS, fused anchor targets + detection losses (csrc/dcn_sample.hip, nms_rotated.hip, anchor_loss.hip).
+"""Deformable-convolution sampling, rotated NMS, fused anchor targets + detection losses, token embedding, distillation from a teacher's top
+logits (csrc/dcn_sample.hip, nms_rotated.hip, anchor_loss.hip, token_embed.hip, topk_distill.hip).
 (Part of omnihd_amd.ops — the tensor-level wrappers over the C ABI; `from omnihd_amd import ops` exposes every name.)"""
 import contextlib
 import ctypes
+import math
 import os
 import weakref
 
 import numpy as np
 import torch
+from torch.autograd.function import once_differentiable
 
 from .._env import env as _env
 from .._lib import check, lib
-from ._core import _on, _ptr, _raw_stream, _same_device, _stream, _want, _workspace
+from ._core import (_TYPE_CODE, _on, _pitch, _ptr, _raw_stream, _rows2d, _same_device, _stream, _want, _want_rows, _workspace)
 
 
 
@@ -168,3 +171,176 @@ def anchor_loss(cls_score, bbox_pred, dir_pred, anchors, gt_boxes, gt_labels, gt
     dense = lambda t: t if (t.is_contiguous() or t.is_contiguous(memory_format=torch.channels_last)) else t.contiguous()
     maps = [dense(t.float()) for t in (cls_score, bbox_pred, dir_pred)]          # differentiable casts: bf16 maps get bf16 gradients
     return _AnchorLoss.apply(maps[0], maps[1], maps[2], anchors, gt_boxes, gt_labels, gt_offsets, meta)
+
+
+# --------------------------------------------------------------------------------------------
+# Token embedding: scaled row lookup, gradient by sorted tokens (csrc/token_embed.hip)
+# --------------------------------------------------------------------------------------------
+def _embed_forward(ids, table, scale, out_dtype):
+    out = torch.empty(ids.shape + (table.shape[1],), dtype=out_dtype, device=table.device)
+    if out.numel():
+        with _on(table.device):
+            check(lib().omnihd_token_embed_fwd(ids.data_ptr(), int(ids.dtype == torch.int64), ids.numel(), table.data_ptr(), _TYPE_CODE[table.dtype],
+                                               _pitch(table), table.shape[0], table.shape[1], scale, out.data_ptr(), _TYPE_CODE[out_dtype],
+                                               _raw_stream()), "omnihd_token_embed_fwd")
+    return out
+
+
+class _TokenEmbed(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, table, ids, scale, padding, out_dtype):
+        ctx.save_for_backward(ids)
+        ctx.meta = (tuple(table.shape), table.dtype, scale, padding)
+        return _embed_forward(ids, table, scale, out_dtype)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        ids, = ctx.saved_tensors
+        (vocab, dim), dtype, scale, padding = ctx.meta
+        dev = g.device
+        g2 = _rows2d(g, dim)
+        grad = torch.empty((vocab, dim), dtype=dtype, device=dev)
+        L, n = lib(), ids.numel()
+        with _on(dev):
+            ws = _workspace(L.omnihd_token_embed_bwd_workspace_bytes(n, dim), dev)
+            check(L.omnihd_token_embed_bwd(ids.data_ptr(), int(ids.dtype == torch.int64), n, g2.data_ptr(), _TYPE_CODE[g2.dtype], _pitch(g2), vocab, dim,
+                                           scale, padding, grad.data_ptr(), _TYPE_CODE[dtype], ws.data_ptr(), ws.numel(), _raw_stream()),
+                  "omnihd_token_embed_bwd")
+        return grad, None, None, None, None
+
+
+def token_embedding(ids, table, scale=1.0, padding_idx=None, out_dtype=None):
+    """``scale * table[ids]``: ids of any shape, int64 or int32; table (vocab, D) fp32, bf16 or fp16 with dense rows (a row pitch is fine).
+    ``out_dtype``: the table's type (the default), or a 16-bit type for an fp32 table.  An id outside [0, vocab) gives a row of NaN.
+    The table's gradient is dense, every row written: the sum of each token's rows in increasing position, in fp32, run-to-run
+    identical; the row of ``padding_idx`` gets none (it is looked up like any other)."""
+    _want_rows(table, "table")
+    if table.dim() != 2 or table.shape[0] < 1 or table.shape[1] < 1:
+        raise ValueError(f"table must be (vocab, D), got {tuple(table.shape)}")
+    if (table.shape[1] > 1 and table.stride(1) != 1) or (table.shape[0] > 1 and table.stride(0) < table.shape[1]):
+        raise ValueError(f"the table's rows must be dense, got strides {tuple(table.stride())}")
+    if not isinstance(ids, torch.Tensor) or ids.dtype not in (torch.int64, torch.int32):
+        raise TypeError("ids must be an int64 or int32 tensor")
+    _same_device(table, ids)
+    out_dtype = table.dtype if out_dtype is None else out_dtype
+    if out_dtype not in _TYPE_CODE or (out_dtype != table.dtype and table.dtype != torch.float32):
+        raise TypeError(f"out_dtype {out_dtype} of a {table.dtype} table: wanted the table's type, or a 16-bit type for an fp32 table")
+    padding = -1
+    if padding_idx is not None:
+        if not -table.shape[0] <= padding_idx < table.shape[0]:
+            raise ValueError(f"padding_idx {padding_idx} is not a row of a table of {table.shape[0]}")
+        padding = int(padding_idx) % table.shape[0]
+    ids = ids.contiguous()
+    if torch.is_grad_enabled() and table.requires_grad:
+        return _TokenEmbed.apply(table, ids, float(scale), padding, out_dtype)
+    return _embed_forward(ids, table, float(scale), out_dtype)
+
+
+# --------------------------------------------------------------------------------------------
+# Distillation from a teacher's top logits (csrc/topk_distill.hip)
+# --------------------------------------------------------------------------------------------
+_DISTILL_MAX_TOP = 256
+
+
+def _distill_call(z, t, ids, weight, avg, meta, grad=None, up=None, skip_if_one=False, want_loss=True):
+    """One launch over the rows: the loss (one number, or one a row) and / or the gradient into `grad`."""
+    temperature, factor, per_row = meta
+    vocab, top = z.shape[-1], t.shape[-1]
+    rows, dev = z.numel() // vocab, z.device
+    z2, t2, i2 = _rows2d(z, vocab), _rows2d(t, top), _rows2d(ids, top)
+    loss = torch.empty(z.shape[:-1] if per_row else (), dtype=torch.float32, device=dev) if want_loss else None
+    L = lib()
+    with _on(dev):
+        ws = _workspace(L.omnihd_topk_distill_workspace_bytes(rows, vocab, top, _TYPE_CODE[z.dtype]), dev) if want_loss and not per_row else None
+        check(L.omnihd_topk_distill(z2.data_ptr(), _TYPE_CODE[z.dtype], _pitch(z2), t2.data_ptr(), _TYPE_CODE[t.dtype], _pitch(t2), i2.data_ptr(),
+                                    int(ids.dtype == torch.int64), _pitch(i2), None if weight is None else weight.data_ptr(), rows, vocab, top,
+                                    temperature, factor, None if avg is None else avg.data_ptr(), None if up is None else up.data_ptr(),
+                                    int(up is not None and per_row), int(skip_if_one), None if grad is None else grad.data_ptr(), vocab,
+                                    loss.data_ptr() if want_loss and per_row else None, loss.data_ptr() if want_loss and not per_row else None,
+                                    None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(), _raw_stream()), "omnihd_topk_distill")
+    return loss
+
+
+class _TopkDistill(torch.autograd.Function):
+    """The forward of a summed loss writes the logits' gradient too, while the row is in registers; the backward returns it, after a launch
+    that writes it again where the gradient arriving at the loss is not 1.  That second form alone (two passes instead of one and a half)
+    serves per-row losses, whose upstream gradient is not known in the forward, stream capture, whose replays may be of the backward
+    alone, and every further backward pass over the same forward."""
+
+    @staticmethod
+    def forward(ctx, z, t, ids, weight, avg, meta):
+        ctx.meta, ctx.fresh = meta, False
+        grad = None
+        if not meta[2] and not torch.cuda.is_current_stream_capturing():
+            grad = torch.empty(z.shape, dtype=z.dtype, device=z.device)
+            ctx.fresh = True
+        loss = _distill_call(z, t, ids, weight, avg, meta, grad)
+        ctx.save_for_backward(z, t, ids, weight, avg, grad)
+        return loss
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, up):
+        z, t, ids, weight, avg, grad = ctx.saved_tensors
+        up = up.to(torch.float32).contiguous()
+        in_place = ctx.fresh and not torch.cuda.is_current_stream_capturing()
+        if in_place:
+            ctx.fresh = False
+        else:
+            grad = torch.empty(z.shape, dtype=z.dtype, device=z.device)
+        _distill_call(z, t, ids, weight, avg, ctx.meta, grad, up, skip_if_one=in_place, want_loss=False)
+        return grad, None, None, None, None, None
+
+
+def topk_distill_loss(logits, teacher_logits, teacher_ids, temperature=1.0, row_weight=None, reduction="mean", avg_factor=None,
+                      loss_weight=1.0):
+    """KL divergence of a student from a teacher of whom the top logits are kept, at a temperature T:
+
+        p = softmax(teacher_logits / T) over the K kept entries,   q = softmax(logits / T) over all V
+        loss = T^2 * sum_k p_k (ln p_k - ln q[teacher_ids_k])                    (per row)
+
+    logits (..., V) fp32, bf16 or fp16 (any row pitch); teacher_logits (..., K) of any of these types and teacher_ids (..., K) int64 or int32,
+    K <= 256.  A negative id marks an empty slot (its logit may hold anything), -inf a slot without mass; the same id may stand in a row twice.
+    An id >= V makes its row's loss and gradient NaN.  row_weight (...) weights the rows: rows of weight 0 and rows without teacher mass add exactly
+    0 with a zero gradient, whatever their logits hold.  reduction: "mean" (over all rows, or divided by ``avg_factor``, a number or a
+    one-element fp32 tensor), "sum", or "none" (the rows' losses); ``loss_weight`` multiplies the result, which is fp32.  No gradient goes
+    to the teacher or the weights."""
+    _want_rows(logits, "logits")
+    _want_rows(teacher_logits, "teacher_logits")
+    if logits.dim() < 1 or logits.shape[-1] < 1:
+        raise ValueError(f"logits must be (..., V), got {tuple(logits.shape)}")
+    if not isinstance(teacher_ids, torch.Tensor) or teacher_ids.dtype not in (torch.int64, torch.int32):
+        raise TypeError("teacher_ids must be an int64 or int32 tensor")
+    lead = tuple(logits.shape[:-1])
+    if teacher_logits.dim() < 1 or teacher_ids.shape != teacher_logits.shape or tuple(teacher_ids.shape[:-1]) != lead:
+        raise ValueError(f"teacher_logits and teacher_ids must be {lead} + (K,), got {tuple(teacher_logits.shape)} and {tuple(teacher_ids.shape)}")
+    if not 1 <= teacher_ids.shape[-1] <= _DISTILL_MAX_TOP:
+        raise ValueError(f"1 to {_DISTILL_MAX_TOP} kept entries a row are supported, got {teacher_ids.shape[-1]}")
+    temperature, loss_weight = float(temperature), float(loss_weight)
+    if not 1e-6 <= temperature <= 1e6:
+        raise ValueError(f"temperature must be in [1e-6, 1e6], got {temperature}")
+    if reduction not in ("mean", "sum", "none"):
+        raise ValueError(f'reduction must be "mean", "sum" or "none", got {reduction!r}')
+    if avg_factor is not None and reduction != "mean":
+        raise ValueError('avg_factor goes with reduction "mean"')
+    avg, rows = None, math.prod(lead)
+    factor = loss_weight
+    if isinstance(avg_factor, torch.Tensor):
+        if avg_factor.numel() != 1:
+            raise ValueError("avg_factor must have one element")
+        avg = avg_factor.detach().to(torch.float32)
+    elif avg_factor is not None:
+        factor = loss_weight / float(avg_factor)
+    elif reduction == "mean":
+        factor = loss_weight / max(rows, 1)
+    if row_weight is not None:
+        if not isinstance(row_weight, torch.Tensor) or tuple(row_weight.shape) != lead:
+            raise ValueError(f"row_weight must be a tensor of shape {lead}")
+        row_weight = row_weight.detach().to(torch.float32).contiguous()
+    _same_device(logits, teacher_logits, teacher_ids, row_weight, avg)
+    meta = (temperature, factor, reduction == "none")
+    teacher_logits = teacher_logits.detach()
+    if torch.is_grad_enabled() and logits.requires_grad:
+        return _TopkDistill.apply(logits, teacher_logits, teacher_ids, row_weight, avg, meta)
+    return _distill_call(logits, teacher_logits, teacher_ids, row_weight, avg, meta)

@@ -1,16 +1,20 @@
-"""BatchNorm epilogues as autograd Functions: frozen (affine + residual + ReLU) and training mode (csrc/affine_act.hip, batch_norm.hip).
+"""BatchNorm epilogues as autograd Functions: frozen (affine + residual + ReLU) and training mode (csrc/affine_act.hip, batch_norm.hip); norms
+before and after a block of token rows (csrc/block_norm.hip).
 (Part of omnihd_amd.ops — the tensor-level wrappers over the C ABI; `from omnihd_amd import ops` exposes every name.)"""
 import contextlib
 import ctypes
+import math
 import os
 import weakref
 
 import numpy as np
 import torch
+from torch.autograd.function import once_differentiable
 
 from .._env import env as _env
 from .._lib import check, lib
-from ._core import FAST_PATHS, _SIZE_CACHE, _f32c, _on, _raw_stream, _rows_view, _want, _wgrad_workspace
+from ._core import (FAST_PATHS, _SIZE_CACHE, _TYPE_CODE, _f32c, _on, _pitch, _raw_stream, _rows2d, _rows_view, _same_device, _want,
+    _want_rows, _wgrad_workspace, _workspace)
 from .policy import _fp32_policy, f16_handover
 from .planes import _alloc_planes, _amax_slot, half_wanted, planes_wanted, tag_half, tag_planes, tag_producer
 
@@ -255,3 +259,156 @@ def bn_train_act(x, weight, bias, running_mean, running_var, momentum, eps, relu
     cl = (lambda t: t.contiguous(memory_format=torch.channels_last)) if x.dim() == 4 else (lambda t: t.contiguous())
     return _BnTrainAct.apply(cl(x), weight, bias, running_mean, running_var, float(momentum), float(eps), bool(relu), group,
                              None if residual is None else cl(residual), bool(unbiased_sync), bool(grad_planes_only))
+
+
+# --------------------------------------------------------------------------------------------
+# Token rows: norms before and after a block, fused with its gate and the residual scale (csrc/block_norm.hip)
+# --------------------------------------------------------------------------------------------
+_BLOCK_MAX_DIM = 16384
+_GATE_NONE, _GATE_ROWS, _GATE_TOKEN, _GATE_FULL = 0, 1, 2, 3
+
+
+def _gate_layout(gate, shape):
+    """(kind, rows that share a gate row) of a gate for rows of `shape` (..., D): one row for all, one for each element of the leading
+    dimensions, one number a row, or one number an element."""
+    gs, d = tuple(gate.shape), shape[-1]
+    if gs == (d,):
+        return _GATE_ROWS, max(1, math.prod(shape[:-1]))
+    if gs == shape:
+        return _GATE_FULL, 1
+    if gs == shape[:-1] + (1,):
+        return _GATE_TOKEN, 1
+    if len(gs) == len(shape) and gs[-1] == d:
+        lead = 0
+        while lead < len(gs) - 1 and gs[lead] == shape[lead]:
+            lead += 1
+        if all(n == 1 for n in gs[lead:-1]):
+            return _GATE_ROWS, max(1, math.prod(shape[lead:-1]))
+    raise ValueError(f"gate of shape {gs} does not fit rows of shape {tuple(shape)}: wanted (D,), the leading dimensions with ones behind "
+                     f"and D, (..., 1), or the rows' own shape")
+
+
+def _block_args(x, y, post, gate, nxt, dim, kind, per_gate):
+    """The leading arguments that the forward and the backward share, and what keeps their memory alive."""
+    x2, y2 = _rows2d(x, dim), None if y is None else _rows2d(y, dim)
+    g2 = None if gate is None else (gate.contiguous().view(-1) if kind == _GATE_TOKEN else _rows2d(gate, dim))
+    post, nxt = (None if w is None else w.contiguous() for w in (post, nxt))
+    code = lambda t: 0 if t is None else _TYPE_CODE[t.dtype]
+    ptr = lambda t: None if t is None else t.data_ptr()
+    act = y if y is not None else x
+    args = (x2.data_ptr(), _pitch(x2), code(x), ptr(y2), 0 if y2 is None else _pitch(y2), code(act), ptr(post), code(post), ptr(g2), code(gate), kind,
+            0 if g2 is None or kind == _GATE_TOKEN else _pitch(g2), per_gate, ptr(nxt), code(nxt))
+    return args, (x2, y2, g2, post, nxt)
+
+
+class _BlockJoin(torch.autograd.Function):
+    """(x, y, post, gate, next) -> (x_out, h); y None: h = norm(x; next) alone.  See include/omnihd_hip.h: omnihd_block_join_fwd."""
+
+    @staticmethod
+    def forward(ctx, x, y, post, gate, nxt, meta):
+        out, h, stats = _block_forward(x, y, post, gate, nxt, meta, True)
+        ctx.save_for_backward(x, y, post, gate, nxt, stats)
+        ctx.meta = meta
+        ctx.set_materialize_grads(False)
+        return out, h
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, d_out, d_h):
+        x, y, post, gate, nxt, stats = ctx.saved_tensors
+        scale, _eps, kind, per_gate, act = ctx.meta
+        want = ctx.needs_input_grad
+        if (d_out is None and d_h is None) or not any(want[:5]):
+            return (None,) * 6
+        dim, dev = x.shape[-1], x.device
+        rows = x.numel() // dim
+        like = lambda t, i: torch.empty(t.shape, dtype=t.dtype, device=dev) if want[i] else None
+        gx, gy, g_post, g_gate, g_next = like(x, 0), like(y, 1), like(post, 2), like(gate, 3), like(nxt, 4)
+        if rows == 0:
+            return tuple(None if g is None else g.zero_() for g in (gx, gy, g_post, g_gate, g_next)) + (None,)
+        args, keep = _block_args(x, y, post, gate, nxt, dim, kind, per_gate)
+        args = args[:5] + (_TYPE_CODE[act],) + args[6:]
+        do2, dh2 = (None if t is None else _rows2d(t, dim) for t in (d_out, d_h))
+        ptr = lambda t: None if t is None else t.data_ptr()
+        L = lib()
+        with _on(dev):
+            ws = _workspace(L.omnihd_block_join_bwd_workspace_bytes(rows, dim, kind, per_gate), dev)
+            check(L.omnihd_block_join_bwd(*args, scale, rows, dim, stats.data_ptr(), ptr(do2), 0 if do2 is None else _pitch(do2), ptr(dh2),
+                                          0 if dh2 is None else _pitch(dh2), ptr(gx), ptr(gy), ptr(g_post), ptr(g_gate), ptr(g_next),
+                                          ws.data_ptr(), ws.numel(), _raw_stream()), "omnihd_block_join_bwd")
+        return gx, gy, g_post, g_gate, g_next, None
+
+
+def _block_forward(x, y, post, gate, nxt, meta, keep_stats):
+    scale, eps, kind, per_gate, act = meta
+    dim, dev = x.shape[-1], x.device
+    rows = x.numel() // dim
+    out = None if y is None else torch.empty(x.shape, dtype=x.dtype, device=dev)
+    h = None if nxt is None else torch.empty(x.shape, dtype=act, device=dev)
+    stats = torch.empty((rows, 2), dtype=torch.float32, device=dev) if keep_stats else None
+    if rows:
+        args, keep = _block_args(x, y, post, gate, nxt, dim, kind, per_gate)
+        args = args[:5] + (_TYPE_CODE[act],) + args[6:]
+        with _on(dev):
+            check(lib().omnihd_block_join_fwd(*args, scale, eps, rows, dim, None if out is None else out.data_ptr(), None if h is None else h.data_ptr(),
+                                              None if stats is None else stats.data_ptr(), _raw_stream()), "omnihd_block_join_fwd")
+    return out, h, stats
+
+
+def _block_checks(x, eps, *weights):
+    _want_rows(x, "x")
+    if not 1 <= x.shape[-1] <= _BLOCK_MAX_DIM:
+        raise ValueError(f"rows of {x.shape[-1]} elements: 1 to {_BLOCK_MAX_DIM} are supported")
+    if not eps >= 1e-30:
+        raise ValueError(f"eps must be at least 1e-30 (a row of zeros has no other scale), got {eps}")
+    for w, name in weights:
+        if w is not None:
+            _want_rows(w, name)
+            if tuple(w.shape) != (x.shape[-1],):
+                raise ValueError(f"{name} must have shape ({x.shape[-1]},), got {tuple(w.shape)}")
+            _same_device(x, w)
+
+
+def block_norm(x, weight, eps=1e-6, out_dtype=None):
+    """The norm in front of a block: ``x * rsqrt(mean(x^2) + eps) * weight`` over the last dimension (up to 16384), x (..., D) fp32, bf16 or
+    fp16, weight (D,) of any of these types; ``out_dtype``: x's (the default), or a 16-bit type for an fp32 x.  Differentiable in both.
+    See ``block_join`` for the norms behind it."""
+    _block_checks(x, eps, (weight, "weight"))
+    if weight is None:
+        raise TypeError("weight must be a tensor")
+    act = x.dtype if out_dtype is None else out_dtype
+    if act not in _TYPE_CODE or (act != x.dtype and x.dtype != torch.float32):
+        raise TypeError(f"out_dtype {act} with {x.dtype} rows: wanted the rows' type, or a 16-bit type for fp32 rows")
+    meta = (1.0, float(eps), _GATE_NONE, 1, act)
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
+        return _BlockJoin.apply(x, None, None, None, weight, meta)[1]
+    return _block_forward(x, None, None, None, weight, meta, False)[1]
+
+
+def block_join(x, y, post_weight=None, gate=None, residual_scale=1.0, next_weight=None, eps=1e-6):
+    """A block's output back into the residual stream, and the norm in front of the next block, in one pass:
+
+        x_out = residual_scale * x + gate * norm(y; post_weight)         (post_weight None: y itself; gate None: 1)
+        h     = norm(x_out; next_weight),   norm(v; w) = v * rsqrt(mean(v^2) + eps) * w
+
+    x (..., D) is the stream, y (the same shape) the block's output; x has y's type or fp32, x_out gets x's type, h gets y's (from the
+    fp32 value of x_out, before its rounding).  gate: (D,), or the leading dimensions of x with ones behind and D (one row a sample), or
+    (..., 1) (a number a row), or y's shape; weights and gate fp32, bf16 or fp16, D up to 16384.  Returns x_out, or (x_out, h) with next_weight.
+    Differentiable in all five, sums over rows in a fixed order; a single token is a row like any other."""
+    _block_checks(x, eps, (post_weight, "post_weight"), (next_weight, "next_weight"))
+    _want_rows(y, "y")
+    if y.shape != x.shape:
+        raise ValueError(f"y must have x's shape {tuple(x.shape)}, got {tuple(y.shape)}")
+    if x.dtype != y.dtype and x.dtype != torch.float32:
+        raise TypeError(f"x must be fp32 or have y's type, got {x.dtype} and {y.dtype}")
+    _same_device(x, y, gate)
+    kind, per_gate = _GATE_NONE, 1
+    if gate is not None:
+        _want_rows(gate, "gate")
+        kind, per_gate = _gate_layout(gate, tuple(x.shape))
+    meta = (float(residual_scale), float(eps), kind, per_gate, y.dtype)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, y, post_weight, gate, next_weight)):
+        out, h = _BlockJoin.apply(x, y, post_weight, gate, next_weight, meta)
+    else:
+        out, h, _ = _block_forward(x, y, post_weight, gate, next_weight, meta, False)
+    return out if next_weight is None else (out, h)
