@@ -696,7 +696,7 @@ int omnihd_token_embed_fwd(const void* ids, int wide_ids, long long n, const voi
                            long long vocab, int dim, float scale, void* out, int out_type, void* stream);
 /* grad[v] = scale * sum of g[i] over the i with ids[i] = v, in increasing order of i, fp32 sums, every row of the dense
  * [vocab][dim] gradient written.  Ids outside [0, vocab) and those equal to `padding` (-1: none) add nothing.        */
-size_t omnihd_token_embed_bwd_workspace_bytes(long long n, int dim);
+size_t omnihd_token_embed_bwd_workspace_bytes(long long n, long long vocab, int dim);
 int omnihd_token_embed_bwd(const void* ids, int wide_ids, long long n, const void* g, int out_type, long long g_stride, long long vocab,
                            int dim, float scale, long long padding, void* grad, int table_type, void* workspace,
                            size_t workspace_bytes, void* stream);
@@ -713,7 +713,7 @@ int omnihd_block_join_fwd(const void* x, long long x_stride, int x_type, const v
                           int dim, void* x_out, void* h_out, float* stats, void* stream);
 /* Gradients of the same inputs (each output may be NULL: not wanted) from dx_out, dh (each may be NULL: zero).  Gradients of
  * post, next and gate have those arrays' types and are dense; fp32 sums in a fixed order.                              */
-size_t omnihd_block_join_bwd_workspace_bytes(long long rows, int dim, int gate_kind, long long rows_per_gate);
+size_t omnihd_block_join_bwd_workspace_bytes(long long rows, int dim, int gate_kind, long long rows_per_gate, int has_y);
 int omnihd_block_join_bwd(const void* x, long long x_stride, int x_type, const void* y, long long y_stride, int act_type,
                           const void* post, int post_type, const void* gate, int gate_type, int gate_kind, long long gate_stride,
                           long long rows_per_gate, const void* next, int next_type, float residual_scale, long long rows, int dim,

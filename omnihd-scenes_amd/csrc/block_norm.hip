@@ -11,7 +11,7 @@
 // gradients in fp32 would carry that rounding (1e-3 of them for bf16 rows).
 //
 // Bound by HBM: 4 rows of D forward, 6 backward, about 50 operations an element in all.  So each row is read once into registers
-// (8 elements a lane and step, TPR lanes a row, TPR chosen so that a lane holds 8 or 16 elements), its one or two sums go over the
+// (8 elements a lane and step, TPR lanes a row, the next row asked for while one is worked on), its one or two sums go over the
 // lanes by DPP (over LDS beyond a wave), and the column sums of the weight gradients stay in registers over all rows that a block
 // walks; only their block sums go through memory ([blocks][2][D] fp32), joined in a fixed order by a second launch.
 // With a gate per channel (or per sample and channel) S = sum_rows t * nh serves both gradients: dgate = S * post, dpost = sum S * gate.
@@ -60,19 +60,33 @@ __global__ __launch_bounds__(threads_of<TPR>()) void k_block_fwd(BlockArgs a) {
       for (int k = 0; k < 8; ++k) gp[j][k] *= g[k];
     }
   }
-  for (long long base = (long long)blockIdx.x * RPB; base < a.rows; base += (long long)gridDim.x * RPB) {
+  typename Raw<TX>::V xr[NV];            // the next row, asked for while this one is worked on
+  typename Raw<TA>::V yr[NV];
+  auto ask = [&](long long row) {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int c = (j * TPR + t) * 8, left = D - c;
+      xr[j] = typename Raw<TX>::V{};
+      if (HASY) yr[j] = typename Raw<TA>::V{};
+      if (row >= a.rows || left <= 0) continue;
+      xr[j] = raw8<ODD>(static_cast<const TX*>(a.x) + row * a.xs + c, left);
+      if (HASY) yr[j] = raw8<ODD>(static_cast<const TA*>(a.y) + row * a.ys + c, left);
+    }
+  };
+  const long long step = (long long)gridDim.x * RPB;
+  ask((long long)blockIdx.x * RPB + sub);
+  for (long long base = (long long)blockIdx.x * RPB; base < a.rows; base += step) {
     const long long row = base + sub;
     const bool act = row < a.rows;
     float x[NV][8], y[NV][8], ry = 1.f, rx = 1.f;
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const int c = (j * TPR + t) * 8, left = D - c;
+    for (int j = 0; j < NV; ++j)
 #pragma unroll
-      for (int k = 0; k < 8; ++k) x[j][k] = y[j][k] = 0.f;
-      if (!act || left <= 0) continue;
-      load8<ODD>(static_cast<const TX*>(a.x) + row * a.xs + c, left, x[j]);
-      if (HASY) load8<ODD>(static_cast<const TA*>(a.y) + row * a.ys + c, left, y[j]);
-    }
+      for (int k = 0; k < 8; ++k) {
+        x[j][k] = (float)xr[j][k];
+        y[j][k] = HASY ? (float)yr[j][k] : 0.f;
+      }
+    ask(row + step);
     if (HASY) {
       if (post) {
         float s = 0.f;
@@ -124,12 +138,15 @@ __global__ __launch_bounds__(threads_of<TPR>()) void k_block_fwd(BlockArgs a) {
   }
 }
 
-// One block: `per_split` rows of one gate row (blockIdx = gate row * splits + split).
+// One block: `per_split` rows of one gate row (blockIdx = gate row * splits + split).  With two vectors a lane (rows beyond 8192) there are
+// not registers for all of it: the weights are read when they are used, no row is asked for ahead, and the column sums are kept in
+// LDS (128 KB) - 2048 rows of 16384 bf16: 312 us with them in registers, which spill.
 template <typename TA, typename TX, int TPR, int NV, bool ODD, bool HASY>
 __global__ __launch_bounds__(threads_of<TPR>()) void k_block_bwd(BlockArgs a) {
   constexpr int TPB = threads_of<TPR>(), RPB = TPB / TPR;
+  constexpr bool LEAN = NV > 1;
   __shared__ float red[32];
-  __shared__ float fold[RPB > 1 ? TPB * NV * 8 : 1];
+  __shared__ float fold[RPB > 1 ? TPB * 8 : 1];
   int turn = 0;
   const int t = threadIdx.x % TPR, sub = threadIdx.x / TPR, D = a.dim;
   const float inv_d = 1.f / (float)D;
@@ -138,82 +155,94 @@ __global__ __launch_bounds__(threads_of<TPR>()) void k_block_bwd(BlockArgs a) {
   long long hi = lo + a.per_split;
   if (hi > first + a.per_gate) hi = first + a.per_gate;
   if (hi > a.rows) hi = a.rows;
-  float gp[NV][8], wn[NV][8], aw[NV][8], au[NV][8];
-#pragma unroll
-  for (int j = 0; j < NV; ++j) {
+  auto weights = [&](int j, float (&gp)[8], float (&wn)[8]) {     // post (times the gate row), next
     const int c = (j * TPR + t) * 8, left = D - c;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) gp[j][k] = wn[j][k] = 1.f, aw[j][k] = au[j][k] = 0.f;
-    if (left <= 0) continue;
-    if (post) load8_any<ODD>(a.post, a.post_type, c, left, gp[j]);
-    if (a.next) load8_any<ODD>(a.next, a.next_type, c, left, wn[j]);
+    for (int k = 0; k < 8; ++k) gp[k] = wn[k] = 1.f;
+    if (left <= 0) return;
+    if (post) load8_any<ODD>(a.post, a.post_type, c, left, gp);
+    if (a.next) load8_any<ODD>(a.next, a.next_type, c, left, wn);
     if (HASY && a.gate_kind == kGateRows) {
       float g[8];
       load8_any<ODD>(a.gate, a.gate_type, grp * a.gs + c, left, g);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) gp[j][k] *= g[k];
+      for (int k = 0; k < 8; ++k) gp[k] *= g[k];
     }
+  };
+  float gph[LEAN ? 1 : NV][8], wnh[LEAN ? 1 : NV][8], awr[LEAN ? 1 : NV][8], aur[LEAN ? 1 : NV][8];
+  extern __shared__ float wide[];        // [2][NV * 8][TPB]
+  auto aw = [&](int j, int k) -> float& { return LEAN ? wide[(j * 8 + k) * TPB + threadIdx.x] : awr[LEAN ? 0 : j][k]; };
+  auto au = [&](int j, int k) -> float& { return LEAN ? wide[(NV * 8 + j * 8 + k) * TPB + threadIdx.x] : aur[LEAN ? 0 : j][k]; };
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    if constexpr (!LEAN) weights(j, gph[j], wnh[j]);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) aw(j, k) = au(j, k) = 0.f;
   }
-  for (long long base = lo; base < hi; base += RPB) {
-    const long long row = base + sub;
-    const bool act = row < hi;
-    float x[NV][8], y[NV][8], d[NV][8], ry = 1.f, rx = 1.f, tok = 1.f;
-    if (act) {
-      const float2 s = *reinterpret_cast<const float2*>(a.stats + 2 * row);
-      ry = s.x; rx = s.y;
-      if (HASY && a.gate_kind == kGateToken) tok = load1_any(a.gate, a.gate_type, row);
-    }
-    float h[NV][8];
+  typename Raw<TX>::V xr[NV], dr[NV];
+  typename Raw<TA>::V yr[NV], hr[NV];
+  float2 stat = make_float2(1.f, 1.f);
+  auto ask = [&](long long row) {
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int c = (j * TPR + t) * 8, left = D - c;
-#pragma unroll
-      for (int k = 0; k < 8; ++k) x[j][k] = y[j][k] = d[j][k] = h[j][k] = 0.f;
-      if (!act || left <= 0) continue;
-      if (a.dh) load8<ODD>(static_cast<const TX*>(a.x) + row * a.xs + c, left, x[j]);
-      if (HASY) load8<ODD>(static_cast<const TA*>(a.y) + row * a.ys + c, left, y[j]);
-      if (a.dxo) load8<ODD>(static_cast<const TX*>(a.dxo) + row * a.dxos + c, left, d[j]);
-      if (a.dh) load8<ODD>(static_cast<const TA*>(a.dh) + row * a.dhs + c, left, h[j]);
+      xr[j] = dr[j] = typename Raw<TX>::V{};
+      yr[j] = hr[j] = typename Raw<TA>::V{};
+      if (row >= hi || left <= 0) continue;
+      if (a.dh) xr[j] = raw8<ODD>(static_cast<const TX*>(a.x) + row * a.xs + c, left);
+      if (HASY) yr[j] = raw8<ODD>(static_cast<const TA*>(a.y) + row * a.ys + c, left);
+      if (HASY && a.dxo) dr[j] = raw8<ODD>(static_cast<const TX*>(a.dxo) + row * a.dxos + c, left);
+      if (a.dh) hr[j] = raw8<ODD>(static_cast<const TA*>(a.dh) + row * a.dhs + c, left);
     }
-    // y := nh; x := xh; d := t
-    if (HASY) {
+    if (row < hi) stat = *reinterpret_cast<const float2*>(a.stats + 2 * row);
+  };
+  if (!LEAN) ask(lo + sub);
+  for (long long base = lo; base < hi; base += RPB) {
+    const long long row = base + sub;
+    const bool act = row < hi;
+    if (LEAN) ask(row);
+    const float ry = stat.x, rx = stat.y;
+    float x[NV][8], y[NV][8], d[NV][8], h[NV][8], tok = 1.f;
 #pragma unroll
-      for (int j = 0; j < NV; ++j)
+    for (int j = 0; j < NV; ++j)
 #pragma unroll
-        for (int k = 0; k < 8; ++k) y[j][k] *= ry;
-    }
-    float full[NV][8];
-    if (HASY && a.gate_kind == kGateFull) {
-#pragma unroll
-      for (int j = 0; j < NV; ++j) {
-        const int c = (j * TPR + t) * 8, left = D - c;
-#pragma unroll
-        for (int k = 0; k < 8; ++k) full[j][k] = 0.f;
-        if (act && left > 0) load8_any<ODD>(a.gate, a.gate_type, row * a.gs + c, left, full[j]);
+      for (int k = 0; k < 8; ++k) {
+        x[j][k] = (float)xr[j][k];
+        y[j][k] = HASY ? (float)yr[j][k] * ry : 0.f;             // nh
+        d[j][k] = HASY ? (float)dr[j][k] : 0.f;
+        h[j][k] = (float)hr[j][k];
       }
-    } else {
+    if (HASY && a.gate_kind == kGateToken && act) tok = load1_any(a.gate, a.gate_type, row);
+    if (!LEAN) ask(row + RPB);
+    auto row_gate = [&](int j, float (&g)[8]) {                  // what multiplies post and a gate row here: a gate of this very row
+      const int c = (j * TPR + t) * 8, left = D - c;
 #pragma unroll
-      for (int j = 0; j < NV; ++j)
-#pragma unroll
-        for (int k = 0; k < 8; ++k) full[j][k] = tok;
-    }
+      for (int k = 0; k < 8; ++k) g[k] = a.gate_kind == kGateFull ? 0.f : tok;
+      if (HASY && a.gate_kind == kGateFull && act && left > 0) load8_any<ODD>(a.gate, a.gate_type, row * a.gs + c, left, g);
+    };
     if (a.dh) {
       float s = 0.f;
 #pragma unroll
-      for (int j = 0; j < NV; ++j)
+      for (int j = 0; j < NV; ++j) {
+        float gl[8], wl[8], g[8];
+        if constexpr (LEAN) weights(j, gl, wl);
+        const float(&gp)[8] = *(LEAN ? &gl : &gph[LEAN ? 0 : j]);
+        const float(&wn)[8] = *(LEAN ? &wl : &wnh[LEAN ? 0 : j]);
+        if (HASY) row_gate(j, g);
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-          const float xn = HASY ? fmaf(y[j][k], gp[j][k] * full[j][k], a.r * x[j][k]) : x[j][k];
-          x[j][k] = xn * rx;
-          au[j][k] = fmaf(h[j][k], x[j][k], au[j][k]);
-          h[j][k] *= wn[j][k];
+          const float xn = HASY ? fmaf(y[j][k], gp[k] * g[k], a.r * x[j][k]) : x[j][k];
+          x[j][k] = xn * rx;                                     // xh
+          au(j, k) = fmaf(h[j][k], x[j][k], au(j, k));
+          h[j][k] *= wn[k];                                      // a
           s = fmaf(h[j][k], x[j][k], s);
         }
+      }
       s = group<TPR>(s, Add(), red, turn) * inv_d;
 #pragma unroll
       for (int j = 0; j < NV; ++j)
 #pragma unroll
-        for (int k = 0; k < 8; ++k) d[j][k] = fmaf(rx, h[j][k] - x[j][k] * s, d[j][k]);
+        for (int k = 0; k < 8; ++k) d[j][k] = fmaf(rx, h[j][k] - x[j][k] * s, d[j][k]);       // t
     }
     if (a.gx) {
 #pragma unroll
@@ -231,14 +260,17 @@ __global__ __launch_bounds__(threads_of<TPR>()) void k_block_bwd(BlockArgs a) {
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int c = (j * TPR + t) * 8, left = D - c;
-      float dg[8];
+      float dg[8], gl[8], wl[8], g[8];
+      if constexpr (LEAN) weights(j, gl, wl);
+      const float(&gp)[8] = *(LEAN ? &gl : &gph[LEAN ? 0 : j]);
+      row_gate(j, g);
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
         const float tn = d[j][k] * y[j][k];
-        aw[j][k] = a.gate_kind == kGateRows ? aw[j][k] + tn : fmaf(tn, full[j][k], aw[j][k]);
-        dg[k] = tn * gp[j][k];
-        s = fmaf(dg[k], a.gate_kind == kGateFull ? full[j][k] : 1.f, s);
-        d[j][k] *= gp[j][k] * full[j][k];           // m
+        aw(j, k) = a.gate_kind == kGateRows ? aw(j, k) + tn : fmaf(tn, g[k], aw(j, k));
+        dg[k] = tn * gp[k];
+        s = fmaf(dg[k], a.gate_kind == kGateFull ? g[k] : 1.f, s);
+        d[j][k] *= gp[k] * g[k];                                 // m
       }
       if (a.gate_kind == kGateFull && a.ggate && act && left > 0) store8_any<ODD>(a.ggate, a.gate_type, row * D + c, left, dg);
     }
@@ -270,7 +302,7 @@ __global__ __launch_bounds__(threads_of<TPR>()) void k_block_bwd(BlockArgs a) {
       const int c = (j * TPR + t) * 8, left = D - c;
       float v[8];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] = which ? au[j][k] : aw[j][k];
+      for (int k = 0; k < 8; ++k) v[k] = which ? au(j, k) : aw(j, k);
       if constexpr (RPB > 1) {           // the block's rows side by side: added in the order of their places
         __syncthreads();
 #pragma unroll
@@ -287,35 +319,42 @@ __global__ __launch_bounds__(threads_of<TPR>()) void k_block_bwd(BlockArgs a) {
   }
 }
 
-// Block sums -> dnext, dpost (tile 0 of the gates) and the gradient of each gate row.  32 columns by 32 places of the blocks.
+// Block sums -> dnext, dpost (grp -1) and the gradient of each gate row.  16 columns by 64 places of the blocks, whose sums are joined in a
+// fixed order; four loads in flight a lane.
 __global__ __launch_bounds__(1024) void k_block_cols(const float* __restrict__ part, int blocks, int splits, int dim, const void* post,
                                                      int post_type, const void* gate, int gate_type, long long gs, int gate_kind,
                                                      void* gpost, void* ggate, void* gnext, int next_type) {
-  __shared__ float s0[32][33], s1[32][33];
-  const int tiles = (dim + 31) / 32, c = (blockIdx.x % tiles) * 32 + (threadIdx.x & 31), place = threadIdx.x >> 5;
+  __shared__ float s0[64][17], s1[64][17];
+  const int tiles = (dim + 15) / 16, c = (blockIdx.x % tiles) * 16 + (threadIdx.x & 15), place = threadIdx.x >> 4;
   const long long grp = (long long)(blockIdx.x / tiles) - 1;
+  const bool gated = gate_kind == kGateRows, many = gated && blocks > splits;
   float w = 0.f, u = 0.f;
   if (c < dim) {
     if (grp < 0) {
-      for (int b = place; b < blocks; b += 32) {
-        if (gpost) {
-          const float v = part[(long long)b * 2 * dim + c];
-          w += gate_kind == kGateRows ? v * load1_any(gate, gate_type, (long long)(b / splits) * gs + c) : v;
+      for (int b = place; b < blocks; b += 256) {
+        float v[4], q[4], f[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int i = b + 64 * k;
+          v[k] = gpost && i < blocks ? part[(long long)i * 2 * dim + c] : 0.f;
+          q[k] = gnext && i < blocks ? part[((long long)i * 2 + 1) * dim + c] : 0.f;
+          f[k] = many && gpost && i < blocks ? load1_any(gate, gate_type, (long long)(i / splits) * gs + c) : 1.f;
         }
-        if (gnext) u += part[((long long)b * 2 + 1) * dim + c];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) { w = fmaf(v[k], f[k], w); u += q[k]; }
       }
     } else {
-      for (int b = place; b < splits; b += 32) w += part[(grp * splits + b) * 2 * dim + c];
+      for (int b = place; b < splits; b += 64) w += part[(grp * splits + b) * 2 * dim + c];
     }
   }
-  s0[place][threadIdx.x & 31] = w;
-  s1[place][threadIdx.x & 31] = u;
+  s0[place][threadIdx.x & 15] = w;
+  s1[place][threadIdx.x & 15] = u;
   __syncthreads();
   if (place == 0 && c < dim) {
-    for (int o = 1; o < 32; ++o) w += s0[o][threadIdx.x], u += s1[o][threadIdx.x];
+    for (int o = 1; o < 64; ++o) w += s0[o][threadIdx.x], u += s1[o][threadIdx.x];
     if (grp >= 0) store1_any(ggate, gate_type, grp * dim + c, post ? w * load1_any(post, post_type, c) : w);
     else {
-      if (gpost) store1_any(gpost, post_type, c, w);
+      if (gpost) store1_any(gpost, post_type, c, gated && !many ? w * load1_any(gate, gate_type, c) : w);
       if (gnext) store1_any(gnext, next_type, c, u);
     }
   }
@@ -323,23 +362,19 @@ __global__ __launch_bounds__(1024) void k_block_cols(const float* __restrict__ p
 
 constexpr int kMaxDim = 16384;
 
-// lanes of a row: 8 elements a lane up to 512 columns, 16 beyond
+// lanes of a row: 8 elements a lane, 16 beyond 8192 columns
 int lanes_of(int dim) {
-  if (dim <= 64) return 8;
-  if (dim <= 128) return 16;
-  if (dim <= 256) return 32;
-  if (dim <= 1024) return 64;
-  if (dim <= 2048) return 128;
-  if (dim <= 4096) return 256;
-  return dim <= 8192 ? 512 : 1024;
+  int l = 8;
+  while (l < 1024 && l * 8 < dim) l *= 2;
+  return l;
 }
 
-// Rows of one gate row are cut into as many blocks as fill the card three times over (a backward block of 256 threads needs about
-// 160 registers: three fit a CU), but no block gets fewer rows than it has places for.
-void split_of(long long rows, int dim, int gate_kind, long long per_gate, long long* groups, int* splits, long long* per_split) {
+// Rows of one gate row are cut into as many blocks as fit the card at once (a backward lane needs up to 128 registers with a block's
+// output, about 64 without: 1024 or 2048 lanes a CU), but no block gets fewer rows than it has places for.
+void split_of(long long rows, int dim, int gate_kind, long long per_gate, bool has_y, long long* groups, int* splits, long long* per_split) {
   const long long per = gate_kind == kGateRows ? per_gate : rows;
   *groups = rows > 0 ? (rows + per - 1) / per : 0;
-  const int tpr = lanes_of(dim), tpb = tpr > 256 ? tpr : 256, rpb = tpb / tpr, want = 3 * kCUs * 256 / tpb;
+  const int tpr = lanes_of(dim), tpb = tpr > 256 ? tpr : 256, rpb = tpb / tpr, want = kCUs * (has_y ? 1024 : 2048) / tpb;
   long long s = (want + *groups - 1) / (*groups > 0 ? *groups : 1), most = (per + rpb - 1) / rpb;
   if (s > most) s = most;
   if (s < 1) s = 1;
@@ -351,7 +386,9 @@ template <typename TA, typename TX, int TPR, int NV, bool ODD, bool HASY>
 void launch(const BlockArgs& a, bool bwd, long long blocks, hipStream_t st) {
   constexpr int TPB = threads_of<TPR>(), RPB = TPB / TPR;
   if (bwd) {
-    hipLaunchKernelGGL((k_block_bwd<TA, TX, TPR, NV, ODD, HASY>), dim3((unsigned)blocks), dim3(TPB), 0, st, a);
+    const size_t wide = NV > 1 ? 2 * NV * 8 * TPB * sizeof(float) : 0;
+    if (wide) (void)hipFuncSetAttribute(reinterpret_cast<const void*>(k_block_bwd<TA, TX, TPR, NV, ODD, HASY>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)wide);
+    hipLaunchKernelGGL((k_block_bwd<TA, TX, TPR, NV, ODD, HASY>), dim3((unsigned)blocks), dim3(TPB), wide, st, a);
   } else {
     long long g = (a.rows + RPB - 1) / RPB, most = (long long)kMaxBlocks * 256 / TPB;
     hipLaunchKernelGGL((k_block_fwd<TA, TX, TPR, NV, ODD, HASY>), dim3((unsigned)(g < most ? g : most)), dim3(TPB), 0, st, a);
@@ -363,11 +400,11 @@ void launch_dim(const BlockArgs& a, bool bwd, long long blocks, hipStream_t st) 
     case 8: return launch<TA, TX, 8, 1, ODD, HASY>(a, bwd, blocks, st);
     case 16: return launch<TA, TX, 16, 1, ODD, HASY>(a, bwd, blocks, st);
     case 32: return launch<TA, TX, 32, 1, ODD, HASY>(a, bwd, blocks, st);
-    case 64: return a.dim <= 512 ? launch<TA, TX, 64, 1, ODD, HASY>(a, bwd, blocks, st) : launch<TA, TX, 64, 2, ODD, HASY>(a, bwd, blocks, st);
-    case 128: return launch<TA, TX, 128, 2, ODD, HASY>(a, bwd, blocks, st);
-    case 256: return launch<TA, TX, 256, 2, ODD, HASY>(a, bwd, blocks, st);
-    case 512: return launch<TA, TX, 512, 2, ODD, HASY>(a, bwd, blocks, st);
-    default: return launch<TA, TX, 1024, 2, ODD, HASY>(a, bwd, blocks, st);
+    case 64: return launch<TA, TX, 64, 1, ODD, HASY>(a, bwd, blocks, st);
+    case 128: return launch<TA, TX, 128, 1, ODD, HASY>(a, bwd, blocks, st);
+    case 256: return launch<TA, TX, 256, 1, ODD, HASY>(a, bwd, blocks, st);
+    case 512: return launch<TA, TX, 512, 1, ODD, HASY>(a, bwd, blocks, st);
+    default: return a.dim <= 8192 ? launch<TA, TX, 1024, 1, ODD, HASY>(a, bwd, blocks, st) : launch<TA, TX, 1024, 2, ODD, HASY>(a, bwd, blocks, st);
   }
 }
 template <typename TA, typename TX>
@@ -423,11 +460,11 @@ extern "C" int omnihd_block_join_fwd(const void* x, long long x_stride, int x_ty
   return run_block(a, x_type, act_type, false, 0, (hipStream_t)stream);
 }
 
-extern "C" size_t omnihd_block_join_bwd_workspace_bytes(long long rows, int dim, int gate_kind, long long rows_per_gate) {
+extern "C" size_t omnihd_block_join_bwd_workspace_bytes(long long rows, int dim, int gate_kind, long long rows_per_gate, int has_y) {
   if (rows <= 0 || dim < 1 || (gate_kind == kGateRows && rows_per_gate < 1)) return 256;
   long long groups, per_split;
   int splits;
-  split_of(rows, dim, gate_kind, rows_per_gate, &groups, &splits, &per_split);
+  split_of(rows, dim, gate_kind, rows_per_gate, has_y, &groups, &splits, &per_split);
   return (size_t)groups * splits * 2 * dim * sizeof(float);
 }
 
@@ -443,8 +480,8 @@ extern "C" int omnihd_block_join_bwd(const void* x, long long x_stride, int x_ty
   hipStream_t st = (hipStream_t)stream;
   long long groups = 0, per_split = 1;
   int splits = 1;
-  split_of(rows, dim, gate_kind, rows_per_gate, &groups, &splits, &per_split);
-  const long long blocks = groups * splits, tiles = (dim + 31) / 32;
+  split_of(rows, dim, gate_kind, rows_per_gate, y != nullptr, &groups, &splits, &per_split);
+  const long long blocks = groups * splits, tiles = (dim + 15) / 16;
   const bool rows_gate = gate_kind == kGateRows && g_gate;
   const bool cols = g_post || g_next || rows_gate;
   OMNIHD_REQUIRE(blocks < (1ll << 31) && tiles * (1 + groups) < (1ll << 31), "grid");

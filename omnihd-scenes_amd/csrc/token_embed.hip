@@ -5,7 +5,7 @@
 //
 // Both are bound by memory: rows gathered and rows written, no arithmetic to speak of.  The gradient's order of summation is fixed
 // by sorting the positions by token, without atomics on values, so it repeats bit for bit:
-//   k_embed_sort  one block per range of table rows.  Its waves each read their part of the ids twice: once to count what is smaller than
+//   k_embed_sort  one block per range of table rows.  Its waves each read their part of the ids: once to count what is smaller than
 //                 the range (this gives the block's place among the sorted positions) and what falls on each row of it (counters in
 //                 LDS, one set a wave), and once to put the positions in place, in order.  So the sort is one launch with no exchange
 //                 between blocks, for n ids read (rows / range) times from the L2.  Rows that got no token are zeroed here.
@@ -19,6 +19,7 @@ namespace {
 using namespace tok;
 
 constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / 64;
+constexpr size_t kCacheBytes = 256u << 20;         // the Infinity Cache: a larger gradient's zero rows are stored past it
 constexpr int kMaxRange = 896;                     // table rows of one sorting block: 16 sets of counters, 56 KB of LDS
 
 template <typename ID> __device__ __forceinline__ bool usable(ID id, long long vocab, long long padding) {
@@ -33,56 +34,74 @@ __global__ __launch_bounds__(256) void k_embed_fwd(const ID* __restrict__ ids, c
   for (long long i = (long long)blockIdx.x * RPB + threadIdx.x / TPR; i < n; i += (long long)gridDim.x * RPB) {
     const long long id = (long long)ids[i];
     const bool ok = id >= 0 && id < vocab;
-    for (int c = t * 8; c < dim; c += TPR * 8) {
-      float v[8];
-      if (ok) {
-        load8<ODD>(table + id * pitch + c, dim - c, v);
+    for (int c = t * 8; c < dim; c += 4 * TPR * 8) {         // four loads in flight a lane
+      float v[4][8];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] *= scale;
-      } else {
-#pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] = __builtin_nanf("");
+      for (int j = 0; j < 4; ++j) {
+        const int at = c + j * TPR * 8;
+        if (at < dim && ok) load8<ODD>(table + id * pitch + at, dim - at, v[j]);
       }
-      store8<ODD>(out + i * dim + c, dim - c, v);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int at = c + j * TPR * 8;
+        if (at >= dim) continue;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[j][k] = ok ? v[j][k] * scale : __builtin_nanf("");
+        store8<ODD, true>(out + i * dim + at, dim - at, v[j]);
+      }
     }
   }
 }
 
-template <typename TT, typename ID, bool ODD>
-__global__ __launch_bounds__(kSortThreads) void k_embed_sort(const ID* __restrict__ ids, long long n, long long vocab, long long padding,
-                                                             int range, int dim, int* __restrict__ keys, int* __restrict__ pos,
+// LISTED: `ids` are those of the block's bucket alone (`span` rows of the table, a multiple of `range`), with their positions
+template <typename TT, typename ID, bool LISTED, bool ODD>
+__global__ __launch_bounds__(kSortThreads) void k_embed_sort(const ID* __restrict__ ids, const int* __restrict__ where,
+                                                             const int* __restrict__ starts, long long n, long long vocab, long long padding,
+                                                             int span, int range, int cap, int dim, int stream, int* __restrict__ keys, int* __restrict__ pos,
                                                              int* __restrict__ used, TT* __restrict__ grad) {
-  extern __shared__ int hist[];                    // [waves][range]
+  extern __shared__ int hist[];                    // [waves][range] counters, [range] empty rows, [waves][cap] positions, [waves][cap] rows
   __shared__ int wave_sum[kSortWaves], empty_rows, smaller[kSortWaves];
   const int w = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const unsigned long long before = (1ull << lane) - 1;
   const long long r0 = (long long)blockIdx.x * range;
   const int rows = (int)(vocab - r0 < range ? vocab - r0 : range);
+  int* empty = hist + kSortWaves * range;
+  int* found_pos = empty + range + w * cap;        // this wave's tokens of the range, in order, as far as there is room
+  short* found_row = reinterpret_cast<short*>(empty + range + kSortWaves * cap) + w * cap;
   for (int i = threadIdx.x; i < kSortWaves * range; i += kSortThreads) hist[i] = 0;
+  if (threadIdx.x == 0) empty_rows = 0;
   __syncthreads();
+  int smaller_buckets = 0;
+  if (LISTED) {
+    const int b = (int)(r0 / span);
+    smaller_buckets = starts[b];
+    n = starts[b + 1] - smaller_buckets;
+    ids += smaller_buckets;
+    where += smaller_buckets;
+  }
   // each wave has a run of the ids, a multiple of 64
   const long long part = ((n + kSortWaves - 1) / kSortWaves + 63) / 64 * 64;
   const long long lo = part * w < n ? part * w : n, hi = lo + part < n ? lo + part : n;
   int* mine = hist + w * range;
-  int less = 0;
-  long long i = lo + lane;
-  for (; i + 448 < hi; i += 512) {                 // eight loads in flight a lane
+  int less = 0, found = 0;                         // (found: the same in all lanes)
+  for (long long b = lo; b < hi; b += 512) {       // eight loads in flight a lane
     ID v[8];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] = ids[i + 64 * k];
+    for (int k = 0; k < 8; ++k) v[k] = b + 64 * k + lane < hi ? ids[b + 64 * k + lane] : (ID)-1;
 #pragma unroll
-    for (int k = 0; k < 8; ++k)
-      if (usable(v[k], vocab, padding)) {
-        const long long d = (long long)v[k] - r0;
-        less += d < 0;
-        if (d >= 0 && d < rows) atomicAdd(mine + d, 1);
+    for (int k = 0; k < 8; ++k) {
+      const bool ok = usable(v[k], vocab, padding);
+      const long long d = (long long)v[k] - r0;
+      less += ok && d < 0;
+      const bool in = ok && d >= 0 && d < rows;
+      const unsigned long long who = __ballot(in);
+      if (who == 0) continue;
+      if (in) {
+        atomicAdd(mine + d, 1);
+        const int at = found + __popcll(who & before);
+        if (at < cap) { found_pos[at] = (int)(b + 64 * k + lane); found_row[at] = (short)d; }
       }
-  }
-  for (; i < hi; i += 64) {
-    const ID v = ids[i];
-    if (usable(v, vocab, padding)) {
-      const long long d = (long long)v - r0;
-      less += d < 0;
-      if (d >= 0 && d < rows) atomicAdd(mine + d, 1);
+      found += __popcll(who);
     }
   }
 #pragma unroll
@@ -93,6 +112,7 @@ __global__ __launch_bounds__(kSortThreads) void k_embed_sort(const ID* __restric
   int total = 0;
   if ((int)threadIdx.x < rows)
     for (int k = 0; k < kSortWaves; ++k) total += hist[k * range + threadIdx.x];
+  if ((int)threadIdx.x < rows && total == 0) empty[atomicAdd(&empty_rows, 1)] = threadIdx.x;   // (their order does not matter)
   int scan = total;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
@@ -101,7 +121,7 @@ __global__ __launch_bounds__(kSortThreads) void k_embed_sort(const ID* __restric
   }
   if (lane == 63) wave_sum[w] = scan;
   __syncthreads();
-  int begin = scan - total, all = 0;
+  int begin = smaller_buckets + scan - total, all = 0;
   for (int k = 0; k < kSortWaves; ++k) {
     begin += smaller[k] + (k < w ? wave_sum[k] : 0);
     all += wave_sum[k];
@@ -113,92 +133,225 @@ __global__ __launch_bounds__(kSortThreads) void k_embed_sort(const ID* __restric
       hist[k * range + threadIdx.x] = begin;
       begin += c;
     }
-  // rows without a token: their numbers, in LDS behind the counters
-  int* empty = hist + kSortWaves * range;
-  if (threadIdx.x == 0) empty_rows = 0;
   __syncthreads();
-  if ((int)threadIdx.x < rows && total == 0) empty[atomicAdd(&empty_rows, 1)] = threadIdx.x;   // (their order does not matter)
-  __syncthreads();
-  if (all > 0) {
-    int bits = 0;
-    while ((1 << bits) < rows) ++bits;
-    for (long long b = lo; b < hi; b += 64) {
-      const long long at = b + lane;
-      const ID v = at < hi ? ids[at] : (ID)-1;
-      const long long d = (long long)v - r0;
-      const bool in = usable(v, vocab, padding) && d >= 0 && d < rows;
-      unsigned long long same = __ballot(in);
-      if (same == 0) continue;
-      for (int k = 0; k < bits; ++k) {             // the lanes with this lane's row
-        const unsigned long long set = __ballot(in && ((d >> k) & 1));
-        same &= ((d >> k) & 1) ? set : ~set;
-      }
-      if (in) {
-        const int place = __popcll(same & ((1ull << lane) - 1));
-        const int from = mine[d];
-        __builtin_amdgcn_wave_barrier();
-        if (place == 0) mine[d] = from + __popcll(same);
-        __builtin_amdgcn_wave_barrier();
-        keys[from + place] = (int)v;
-        pos[from + place] = (int)at;
+  int bits = 0;
+  while ((1 << bits) < rows) ++bits;
+  // 64 tokens of this wave in order: each to the place that its row has reached
+  auto place = [&](bool in, int d, int at) {
+    unsigned long long same = __ballot(in);
+    for (int k = 0; k < bits; ++k) {               // the lanes with this lane's row
+      const unsigned long long set = __ballot(in && ((d >> k) & 1));
+      same &= ((d >> k) & 1) ? set : ~set;
+    }
+    if (in) {
+      const int nth = __popcll(same & before), from = mine[d];
+      __builtin_amdgcn_wave_barrier();
+      if (nth == 0) mine[d] = from + __popcll(same);
+      __builtin_amdgcn_wave_barrier();
+      keys[from + nth] = (int)(r0 + d);
+      pos[from + nth] = LISTED ? where[at] : at;
+    }
+  };
+  if (found <= cap) {
+    for (int b = 0; b < found; b += 64) {
+      const bool in = b + lane < found;
+      place(in, in ? found_row[b + lane] : 0, in ? found_pos[b + lane] : 0);
+    }
+  } else {                                         // a crowded range: the ids once more
+    for (long long b = lo; b < hi; b += 512) {
+      ID v[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = b + 64 * k + lane < hi ? ids[b + 64 * k + lane] : (ID)-1;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const long long d = (long long)v[k] - r0;
+        const bool in = usable(v[k], vocab, padding) && d >= 0 && d < rows;
+        if (__ballot(in) != 0) place(in, in ? (int)d : 0, (int)(b + 64 * k + lane));
       }
     }
   }
   for (int e = w; e < empty_rows; e += kSortWaves) {
     TT* row = grad + (r0 + empty[e]) * dim;
     const float zero[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    for (int c = lane * 8; c < dim; c += 512) store8<ODD>(row + c, dim - c, zero);
+    if (stream)
+      for (int c = lane * 8; c < dim; c += 512) store8<ODD, true>(row + c, dim - c, zero);
+    else
+      for (int c = lane * 8; c < dim; c += 512) store8<ODD>(row + c, dim - c, zero);
   }
 }
 
-// LANES lanes own one chunk x slab of LANES * 8 columns.
+// Many ids: first into buckets of `span` table rows, in order, so that each sorting block reads its bucket's alone.  Blocks of 4 waves, a
+// chunk of ids each: count, offsets (one block a bucket: where each chunk's share of it begins), place.
+constexpr int kChunkIds = 4096, kMaxBuckets = 2048;
+
+template <typename ID>
+__global__ __launch_bounds__(256) void k_embed_count(const ID* __restrict__ ids, long long n, long long vocab, long long padding, int span,
+                                                     int buckets, int chunks, int* __restrict__ counts) {
+  __shared__ int hist[kMaxBuckets];
+  for (int b = threadIdx.x; b < buckets; b += 256) hist[b] = 0;
+  __syncthreads();
+  const long long lo = (long long)blockIdx.x * kChunkIds;
+#pragma unroll 4
+  for (int i = threadIdx.x; i < kChunkIds; i += 256) {
+    const ID v = lo + i < n ? ids[lo + i] : (ID)-1;
+    if (usable(v, vocab, padding)) atomicAdd(hist + (unsigned)v / (unsigned)span, 1);
+  }
+  __syncthreads();
+  for (int b = threadIdx.x; b < buckets; b += 256) counts[(long long)b * chunks + blockIdx.x] = hist[b];
+}
+
+__global__ __launch_bounds__(256) void k_embed_offsets(int chunks, int* __restrict__ counts, int* __restrict__ totals) {
+  __shared__ int wave_sum[4];
+  const int w = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  int* mine = counts + (long long)blockIdx.x * chunks;
+  int run = 0;
+  for (int b = 0; b < chunks; b += 256) {
+    const int i = b + threadIdx.x, v = i < chunks ? mine[i] : 0;
+    int scan = v;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int up = __shfl_up(scan, o, 64);
+      if (lane >= o) scan += up;
+    }
+    if (lane == 63) wave_sum[w] = scan;
+    __syncthreads();
+    int at = run + scan - v;
+    for (int k = 0; k < 4; ++k) {
+      at += k < w ? wave_sum[k] : 0;
+      run += wave_sum[k];
+    }
+    if (i < chunks) mine[i] = at;
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) totals[blockIdx.x] = run;
+}
+
+template <typename ID>
+__global__ __launch_bounds__(256) void k_embed_place(const ID* __restrict__ ids, long long n, long long vocab, long long padding, int span,
+                                                     int buckets, int chunks, const int* __restrict__ offsets, const int* __restrict__ totals,
+                                                     int* __restrict__ starts, int* __restrict__ out_ids, int* __restrict__ out_pos) {
+  __shared__ int hist[4][kMaxBuckets], wave_sum[4];
+  const int w = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const unsigned long long before = (1ull << lane) - 1;
+  for (int b = threadIdx.x; b < 4 * kMaxBuckets; b += 256) (&hist[0][0])[b] = 0;
+  __syncthreads();
+  const long long lo = (long long)blockIdx.x * kChunkIds + w * (kChunkIds / 4);
+#pragma unroll 4
+  for (int i = lane; i < kChunkIds / 4; i += 64) {
+    const ID v = lo + i < n ? ids[lo + i] : (ID)-1;
+    if (usable(v, vocab, padding)) atomicAdd(&hist[w][(unsigned)v / (unsigned)span], 1);
+  }
+  __syncthreads();
+  // eight neighbouring buckets a thread: where each begins, this chunk's and each wave's share of it
+  constexpr int PER = kMaxBuckets / 256;
+  int total[PER], sum = 0;
+#pragma unroll
+  for (int k = 0; k < PER; ++k) {
+    const int b = threadIdx.x * PER + k;
+    total[k] = b < buckets ? totals[b] : 0;
+    sum += total[k];
+  }
+  int scan = sum;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int up = __shfl_up(scan, o, 64);
+    if (lane >= o) scan += up;
+  }
+  if (lane == 63) wave_sum[w] = scan;
+  __syncthreads();
+  int begin = scan - sum;
+  for (int k = 0; k < w; ++k) begin += wave_sum[k];
+#pragma unroll
+  for (int k = 0; k < PER; ++k) {
+    const int b = threadIdx.x * PER + k;
+    if (b < buckets) {
+      if (blockIdx.x == 0) {
+        starts[b] = begin;
+        if (b == buckets - 1) starts[buckets] = begin + total[k];
+      }
+      int at = begin + offsets[(long long)b * chunks + blockIdx.x];
+      for (int q = 0; q < 4; ++q) {
+        const int c = hist[q][b];
+        hist[q][b] = at;
+        at += c;
+      }
+    }
+    begin += total[k];
+  }
+  __syncthreads();
+  int bits = 0;
+  while ((1 << bits) < buckets) ++bits;
+  for (int i = lane; i < kChunkIds / 4; i += 64) {
+    const ID v = lo + i < n ? ids[lo + i] : (ID)-1;
+    const bool in = usable(v, vocab, padding);
+    const unsigned b = in ? (unsigned)v / (unsigned)span : 0;
+    unsigned long long same = __ballot(in);
+    for (int k = 0; k < bits; ++k) {
+      const unsigned long long set = __ballot(in && ((b >> k) & 1));
+      same &= ((b >> k) & 1) ? set : ~set;
+    }
+    if (in) {
+      const int nth = __popcll(same & before), from = hist[w][b];
+      __builtin_amdgcn_wave_barrier();
+      if (nth == 0) hist[w][b] = from + __popcll(same);
+      __builtin_amdgcn_wave_barrier();
+      out_ids[from + nth] = (int)v;
+      out_pos[from + nth] = (int)(lo + i);
+    }
+  }
+}
+
+// LANES lanes own one chunk x slab of LANES * 8 columns.  They hold LANES sorted positions at a time, one each, so the rows' addresses
+// are there before the rows are asked for: eight row loads in flight.
 template <typename TT, typename TO, int LANES, bool ODD>
 __global__ __launch_bounds__(256) void k_embed_sum(const TO* __restrict__ g, long long pitch, const int* __restrict__ keys,
                                                    const int* __restrict__ pos, const int* __restrict__ used, int chunk, int slabs, int dim,
                                                    float scale, TT* __restrict__ grad, float* __restrict__ parts) {
-  const int n = *used;
+  const int n = *used, lane = threadIdx.x % LANES;
   const long long unit = (long long)blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
   const long long c = unit / slabs;
-  const int col = (int)(unit % slabs) * LANES * 8 + (threadIdx.x % LANES) * 8, left = dim - col;
+  const int col = (int)(unit % slabs) * LANES * 8 + lane * 8, left = dim - col;
   const long long lo = c * chunk;
-  if (lo >= n || left <= 0) return;
+  if (lo >= n) return;                             // (the same in all lanes of a unit)
   const int hi = (int)(lo + chunk < n ? lo + chunk : n);
-  const bool open = lo > 0 && keys[lo - 1] == keys[lo];     // the first run began in an earlier chunk
-  bool first = true;
+  const int earlier = lo > 0 ? keys[lo - 1] : -1, later = hi < n ? keys[hi] : -1;
+  bool first = true, open = false;                 // open: the chunk's first run began in an earlier one
   float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  int i = (int)lo;
-  while (i < hi) {
-    // four rows ahead: the loads of one step do not wait for one another
-    const int m = hi - i < 4 ? hi - i : 4;
-    int key[4];
-    float v[4][8];
+  auto at = [&](int v, int i) { return LANES == 64 ? __builtin_amdgcn_readlane(v, i) : __shfl(v, i, LANES); };
+  for (int b = (int)lo; b < hi; b += LANES) {
+    const int m = hi - b < LANES ? hi - b : LANES;
+    const int mykey = lane < m ? keys[b + lane] : -1, mypos = lane < m ? pos[b + lane] : 0;
+    const int beyond = b + m < hi ? keys[b + m] : later;      // the key behind these
+    if (b == lo) open = at(mykey, 0) == earlier;
+    for (int i = 0; i < m; i += 8) {
+      float v[8][8];
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
-      if (k < m) {
-        key[k] = keys[i + k];
-        load8<ODD>(g + (long long)pos[i + k] * pitch + col, left, v[k]);
+      for (int k = 0; k < 8; ++k)
+        if (i + k < m) {
+          const long long p = at(mypos, i + k);
+          if (left > 0) load8<ODD>(g + p * pitch + col, left, v[k]);
+        }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        if (i + k >= m) break;
+#pragma unroll
+        for (int q = 0; q < 8; ++q) acc[q] += v[k][q];
+        const int key = at(mykey, i + k), next = i + k + 1 < m ? at(mykey, i + k + 1) : beyond;
+        const bool ends = b + i + k + 1 == hi;
+        if (key == next && !ends) continue;
+        if ((first && open) || key == next) {      // a part of a run across chunks: its end (0) or its beginning (1)
+          if (left > 0) store8<ODD>(parts + (2 * c + (first && open ? 0 : 1)) * dim + col, left, acc);
+        } else {
+          float o[8];
+#pragma unroll
+          for (int q = 0; q < 8; ++q) o[q] = acc[q] * scale;
+          if (left > 0) store8<ODD>(grad + (long long)key * dim + col, left, o);
+        }
+        first = false;
+#pragma unroll
+        for (int q = 0; q < 8; ++q) acc[q] = 0.f;
       }
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      if (k >= m) break;
-#pragma unroll
-      for (int q = 0; q < 8; ++q) acc[q] += v[k][q];
-      const int at = i + k;
-      const bool more = at + 1 < n && keys[at + 1] == key[k];
-      if (more && at + 1 < hi) continue;
-      if ((first && open) || more) {               // a part of a run across chunks: its end (0) or its beginning (1)
-        store8<ODD>(parts + (2 * c + (first && open ? 0 : 1)) * dim + col, left, acc);
-      } else {
-        float o[8];
-#pragma unroll
-        for (int q = 0; q < 8; ++q) o[q] = acc[q] * scale;
-        store8<ODD>(grad + (long long)key[k] * dim + col, left, o);
-      }
-      first = false;
-#pragma unroll
-      for (int q = 0; q < 8; ++q) acc[q] = 0.f;
     }
-    i += m;
   }
 }
 
@@ -249,10 +402,15 @@ int lanes_for(int dim, int most) {
   return l;
 }
 
-// rows of a sorting block: one block a CU, until the counters fill the LDS
+// rows of a sorting block: two blocks a CU, until the counters fill the LDS
 int range_for(long long vocab) {
-  long long r = (vocab + kCUs - 1) / kCUs;
+  long long r = (vocab + 2 * kCUs - 1) / (2 * kCUs);
   return (int)(r > kMaxRange ? kMaxRange : r < 1 ? 1 : r);
+}
+// tokens that a wave of a sorting block can keep: what is left of 64 KB, no more than 256
+int cap_for(int range) {
+  const int c = (64000 - (kSortWaves + 1) * range * 4) / (kSortWaves * 6);
+  return (c > 256 ? 256 : c) & ~1;
 }
 // sorted positions of one chunk: short ones while few, so that they fill the card; at most some thousands of parts to join
 int chunk_for(long long n) {
@@ -261,21 +419,40 @@ int chunk_for(long long n) {
   return c;
 }
 
-struct BwdWs { size_t keys, pos, used, parts, total; long long chunks; };
-BwdWs bwd_ws(long long n, int dim) {
-  BwdWs w;
+// From here on the ids are put into buckets first: three more launches, but no block reads all of them.
+constexpr long long kBucketIds = 1 << 17;
+int span_for(long long vocab) {
+  const long long range = range_for(vocab), ranges = (vocab + range - 1) / range;
+  return (int)(range * ((ranges + kMaxBuckets - 1) / kMaxBuckets));
+}
+
+struct BwdWs { size_t keys, pos, used, parts, ids, where, starts, totals, counts, total; long long chunks, buckets, id_chunks; };
+BwdWs bwd_ws(long long n, long long vocab, int dim) {
+  BwdWs w{};
+  size_t at = 0;
+  auto take = [&](size_t bytes) { const size_t from = at; at += align_up(bytes, 256); return from; };
   w.chunks = (n + chunk_for(n) - 1) / chunk_for(n);
-  w.keys = 0;
-  w.pos = align_up((size_t)n * 4, 256);
-  w.used = w.pos + align_up((size_t)n * 4, 256);
-  w.parts = w.used + 256;
-  w.total = w.parts + (w.chunks > 1 ? (size_t)w.chunks * 2 * dim * sizeof(float) : 0);
+  w.keys = take((size_t)n * 4);
+  w.pos = take((size_t)n * 4);
+  w.used = take(4);
+  w.parts = take(w.chunks > 1 ? (size_t)w.chunks * 2 * dim * sizeof(float) : 0);
+  if (n >= kBucketIds) {
+    w.buckets = (vocab + span_for(vocab) - 1) / span_for(vocab);
+    w.id_chunks = (n + kChunkIds - 1) / kChunkIds;
+    w.ids = take((size_t)n * 4);
+    w.where = take((size_t)n * 4);
+    w.starts = take((size_t)(w.buckets + 1) * 4);
+    w.totals = take((size_t)w.buckets * 4);
+    w.counts = take((size_t)w.buckets * w.id_chunks * 4);
+  }
+  w.total = at;
   return w;
 }
 
 template <typename TT, typename TO, typename ID, bool ODD>
 int fwd(const void* ids, const void* table, long long pitch, long long vocab, long long n, int dim, float scale, void* out, hipStream_t st) {
-  const int tpr = lanes_for(dim, 256);
+  // few rows: as many lanes as a row has use for; many: a wave a row at most, whose four loads a lane are in flight together
+  const int tpr = lanes_for(dim, n < 4096 ? 256 : 64);
   const long long rpb = 256 / tpr, g = (n + rpb - 1) / rpb, most = 64ll * kMaxBlocks;
   const dim3 grid((unsigned)(g < most ? g : most)), block(256);
 #define OMNIHD_EMBED_FWD(L) hipLaunchKernelGGL((k_embed_fwd<TT, TO, ID, L, ODD>), grid, block, 0, st, static_cast<const ID*>(ids), \
@@ -297,10 +474,25 @@ int bwd(const void* ids, const void* g, long long pitch, long long vocab, long l
         char* ws, const BwdWs& at, hipStream_t st) {
   int *keys = reinterpret_cast<int*>(ws + at.keys), *pos = reinterpret_cast<int*>(ws + at.pos), *used = reinterpret_cast<int*>(ws + at.used);
   float* parts = reinterpret_cast<float*>(ws + at.parts);
-  const int range = range_for(vocab), chunk = chunk_for(n);
-  hipLaunchKernelGGL((k_embed_sort<TT, ID, ODD>), dim3((unsigned)((vocab + range - 1) / range)), dim3(kSortThreads),
-                     (size_t)(kSortWaves + 1) * range * sizeof(int), st, static_cast<const ID*>(ids), n, vocab, padding, range, dim, keys,
-                     pos, used, static_cast<TT*>(grad));
+  const int range = range_for(vocab), cap = cap_for(range), chunk = chunk_for(n);
+  const dim3 sorters((unsigned)((vocab + range - 1) / range));
+  const size_t lds = (size_t)(kSortWaves + 1) * range * sizeof(int) + (size_t)kSortWaves * cap * 6;
+  const int stream = (size_t)vocab * dim * sizeof(TT) > kCacheBytes;
+  if (at.buckets) {
+    const int span = span_for(vocab), buckets = (int)at.buckets, chunks = (int)at.id_chunks;
+    int *listed = reinterpret_cast<int*>(ws + at.ids), *where = reinterpret_cast<int*>(ws + at.where), *starts = reinterpret_cast<int*>(ws + at.starts);
+    int *totals = reinterpret_cast<int*>(ws + at.totals), *counts = reinterpret_cast<int*>(ws + at.counts);
+    const ID* from = static_cast<const ID*>(ids);
+    hipLaunchKernelGGL((k_embed_count<ID>), dim3(chunks), dim3(256), 0, st, from, n, vocab, padding, span, buckets, chunks, counts);
+    hipLaunchKernelGGL(k_embed_offsets, dim3(buckets), dim3(256), 0, st, chunks, counts, totals);
+    hipLaunchKernelGGL((k_embed_place<ID>), dim3(chunks), dim3(256), 0, st, from, n, vocab, padding, span, buckets, chunks, counts, totals, starts,
+                       listed, where);
+    hipLaunchKernelGGL((k_embed_sort<TT, int, true, ODD>), sorters, dim3(kSortThreads), lds, st, listed, where, starts, n, vocab, padding, span, range,
+                       cap, dim, stream, keys, pos, used, static_cast<TT*>(grad));
+  } else {
+    hipLaunchKernelGGL((k_embed_sort<TT, ID, false, ODD>), sorters, dim3(kSortThreads), lds, st, static_cast<const ID*>(ids), nullptr, nullptr, n, vocab,
+                       padding, 1, range, cap, dim, stream, keys, pos, used, static_cast<TT*>(grad));
+  }
   if (n > 0) {
     const int l = lanes_for(dim, 64), slabs = (dim + l * 8 - 1) / (l * 8);
     const long long units = at.chunks * slabs, per = 256 / l;
@@ -355,8 +547,8 @@ extern "C" int omnihd_token_embed_fwd(const void* ids, int wide_ids, long long n
 #undef OMNIHD_EMBED_ODD
 }
 
-extern "C" size_t omnihd_token_embed_bwd_workspace_bytes(long long n, int dim) {
-  return n < 0 || dim < 1 ? 0 : bwd_ws(n, dim).total;
+extern "C" size_t omnihd_token_embed_bwd_workspace_bytes(long long n, long long vocab, int dim) {
+  return n < 0 || n >= (1ll << 31) || vocab < 1 || vocab >= (1ll << 31) || dim < 1 ? 0 : bwd_ws(n, vocab, dim).total;
 }
 
 extern "C" int omnihd_token_embed_bwd(const void* ids, int wide_ids, long long n, const void* g, int out_type, long long g_stride,
@@ -364,7 +556,7 @@ extern "C" int omnihd_token_embed_bwd(const void* ids, int wide_ids, long long n
                                       void* workspace, size_t workspace_bytes, void* stream) {
   OMNIHD_EMBED_CHECKS;
   OMNIHD_REQUIRE(grad && workspace && (n == 0 || (ids && g && g_stride >= dim)), "null pointer or short rows");
-  const BwdWs at = bwd_ws(n, dim);
+  const BwdWs at = bwd_ws(n, vocab, dim);
   if (workspace_bytes < at.total) { set_error("token_embed_bwd: workspace %zu < required %zu", workspace_bytes, at.total); return OMNIHD_ERR_WORKSPACE; }
   OMNIHD_REQUIRE(at.chunks * ((dim + 63) / 64) < (1ll << 31), "grid");
   hipStream_t st = (hipStream_t)stream;

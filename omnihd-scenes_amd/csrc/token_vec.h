@@ -12,8 +12,6 @@ enum { kF32 = 0, kBF16 = 1, kF16 = 2 };          // omnihd_hip.h: element type c
 inline bool type_ok(int t) { return t == kF32 || t == kBF16 || t == kF16; }
 inline int type_size(int t) { return t == kF32 ? 4 : 2; }
 
-template <typename T> struct TypeSize { static constexpr int value = sizeof(T); };
-
 // eight elements from p; `left` (> 0) elements of the row remain from p on.  Missing ones read as `fill`.
 template <bool ODD, typename T>
 __device__ __forceinline__ void load8(const T* __restrict__ p, int left, float (&v)[8], float fill = 0.f) {
@@ -29,7 +27,21 @@ __device__ __forceinline__ void load8(const T* __restrict__ p, int left, float (
   }
 }
 
+// the same kept as they are (a row that is asked for ahead of its use), missing ones 0
+template <typename T> struct Raw { typedef T V __attribute__((ext_vector_type(8))); };
 template <bool ODD, typename T>
+__device__ __forceinline__ typename Raw<T>::V raw8(const T* __restrict__ p, int left) {
+  typedef typename Raw<T>::V V;
+  typedef V W __attribute__((aligned(ODD ? sizeof(T) : 16)));
+  if (!ODD || left >= 8) return *reinterpret_cast<const W*>(p);
+  V v;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) v[k] = k < left ? p[k] : (T)0.f;
+  return v;
+}
+
+// STREAM: past the caches, for an output that they would not hold anyway
+template <bool ODD, bool STREAM = false, typename T>
 __device__ __forceinline__ void store8(T* __restrict__ p, int left, const float (&v)[8]) {
   if (!ODD || left >= 8) {
     typedef T V __attribute__((ext_vector_type(8)));
@@ -37,7 +49,8 @@ __device__ __forceinline__ void store8(T* __restrict__ p, int left, const float 
     V raw;
 #pragma unroll
     for (int k = 0; k < 8; ++k) raw[k] = (T)v[k];      // round to nearest even
-    *reinterpret_cast<W*>(p) = raw;
+    if (STREAM) __builtin_nontemporal_store(raw, reinterpret_cast<W*>(p));
+    else *reinterpret_cast<W*>(p) = raw;
   } else {
 #pragma unroll
     for (int k = 0; k < 8; ++k)

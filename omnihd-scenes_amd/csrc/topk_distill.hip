@@ -10,7 +10,7 @@
 //
 // Bound by HBM at large V: V read, V written; about 15 operations an element (two exponentials among them) take half as long.  So a row
 // is read once into registers (16 bytes a lane and step), its maximum and its sum of exponentials go over the lanes that share it, and the
-// gradient is written from the registers.  Rows beyond 64 K (16-bit) entries are read twice, the second time out of the caches.  All in base 2:
+// gradient is written from the registers.  Rows beyond 128 K (16-bit) entries are read twice, the second time out of the caches.  All in base 2:
 // exp2(z * c - m * c), c = log2(e) / T, one fused multiply-add with a single rounding of the difference; sums in fp32.
 // The few entries that the teacher names are written again behind the row's own stores, from their own p sums (slots with the same id are
 // summed by the first of them, so an id may stand in a row more than once).
@@ -51,11 +51,12 @@ __device__ __forceinline__ typename Pack<T>::V load_pack(const T* __restrict__ p
   for (int k = 0; k < Pack<T>::n; ++k) v[k] = k < left ? p[k] : (T)-__builtin_inff();
   return v;
 }
+// (past the caches: the gradient of a large vocabulary is read long after it is written - 1021 x 50021 fp16: 58 us, 49 with it)
 template <bool ODD, typename T>
 __device__ __forceinline__ void store_pack(T* __restrict__ p, int left, const typename Pack<T>::V& v) {
   typedef typename Pack<T>::V V;
   typedef V W __attribute__((aligned(ODD ? sizeof(T) : 16)));
-  if (!ODD || left >= Pack<T>::n) { *reinterpret_cast<W*>(p) = v; return; }
+  if (!ODD || left >= Pack<T>::n) { __builtin_nontemporal_store(v, reinterpret_cast<W*>(p)); return; }
 #pragma unroll
   for (int k = 0; k < Pack<T>::n; ++k)
     if (k < left) p[k] = v[k];
@@ -69,16 +70,16 @@ __device__ __forceinline__ float rounded(float v) { asm volatile("" : "+v"(v)); 
 
 // TPR lanes a row; NV steps of 16 bytes a lane in registers, or (NV = 0) the row is read twice.
 template <typename T, int TPR, int NV, bool ODD>
-__global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_distill_rows(DistillArgs a) {
+__global__ __launch_bounds__(TPR > 256 ? TPR : 256, TPR > 256 ? 4 : 1) void k_distill_rows(DistillArgs a) {
   constexpr int TPB = TPR > 256 ? TPR : 256, RPB = TPB / TPR, VE = Pack<T>::n, SL = TPR < 64 ? TPR : 64, KEEP = NV ? NV : 1;
   typedef typename Pack<T>::V V;
   __shared__ float red[32], row_coef[RPB], row_sum[RPB];
-  extern __shared__ float slots[];       // [RPB][2][K]: ids and teacher values
+  extern __shared__ float slots[];       // [RPB][3][K]: ids, teacher's and student's values
   if (a.skip_if_one && *a.up == 1.f) return;
   int turn = 0;
   const int t = threadIdx.x % TPR, sub = threadIdx.x / TPR, K = a.top;
-  int* sid = reinterpret_cast<int*>(slots) + sub * 2 * K;
-  float* st = slots + sub * 2 * K + K;
+  int* sid = reinterpret_cast<int*>(slots) + sub * 3 * K;
+  float *st = slots + sub * 3 * K + K, *sz = st + K;
   const float c = 1.44269504088896341f / a.temperature, base = factor_of(a);
   float total = 0.f;
   for (long long first = (long long)blockIdx.x * RPB; first < a.rows; first += (long long)gridDim.x * RPB) {
@@ -86,6 +87,17 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_distill_rows(DistillA
     const bool act = row < a.rows;
     const T* z = static_cast<const T*>(a.z) + (act ? row : 0) * a.zs;
     const float w = !act ? 0.f : a.w ? a.w[row] : 1.f;
+    // the row is asked for first: the teacher's slots are worked on while it is on its way
+    V keep[KEEP];
+    if constexpr (NV > 0) {
+      if (w != 0.f) {
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+          const int at = (j * TPR + t) * VE, left = a.vocab - at;
+          if (left > 0) keep[j] = load_pack<ODD>(z + at, left);
+        }
+      }
+    }
     // the teacher: lanes t < SL of the row's first wave
     float coef = 0.f, mt = -__builtin_inff(), ls = 0.f;
     if (TPR <= 64 || t < 64) {
@@ -95,8 +107,10 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_distill_rows(DistillA
           const long long id = id_at(a, row * a.is + k);
           const float v = id < 0 ? -__builtin_inff() : load1_any(a.t, a.t_type, row * a.ts + k);
           bad |= id >= a.vocab;
-          sid[k] = id < 0 || id >= a.vocab ? -1 : (int)id;
+          const bool fits = id >= 0 && id < a.vocab;
+          sid[k] = fits ? (int)id : -1;
           st[k] = v;
+          sz[k] = fits ? (float)z[id] : 0.f;
           mt = MaxNan()(mt, v);
         }
       mt = lanes<SL>(mt, MaxNan());
@@ -117,26 +131,26 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_distill_rows(DistillA
       if (TPR > 64 && t == 0) row_coef[sub] = coef;
     }
     // the row's maximum and sum
-    V keep[KEEP];
     float m = -__builtin_inff(), s = 0.f, own_mc = 0.f;
     if (w != 0.f) {
       if constexpr (NV > 0) {
-#pragma unroll
-        for (int j = 0; j < NV; ++j) {
-          const int at = (j * TPR + t) * VE, left = a.vocab - at;
-          if (left > 0) keep[j] = load_pack<ODD>(z + at, left);
-        }
 #pragma unroll
         for (int j = 0; j < NV; ++j)
           if ((j * TPR + t) * VE < a.vocab)
 #pragma unroll
             for (int k = 0; k < VE; ++k) m = fmaxf(m, (float)keep[j][k]);
       } else {
-        for (int at = t * VE; at < a.vocab; at += TPR * VE) {
-          const V v = load_pack<ODD>(z + at, a.vocab - at);
-          float big = (float)v[0];
+        for (int at = t * VE; at < a.vocab; at += 4 * TPR * VE) {        // four loads in flight a lane
+          V v[4];
+          float big = -__builtin_inff();
 #pragma unroll
-          for (int k = 1; k < VE; ++k) big = fmaxf(big, (float)v[k]);
+          for (int j = 0; j < 4; ++j)
+            if (at + j * TPR * VE < a.vocab) v[j] = load_pack<ODD>(z + at + j * TPR * VE, a.vocab - at - j * TPR * VE);
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (at + j * TPR * VE < a.vocab)
+#pragma unroll
+              for (int k = 0; k < VE; ++k) big = fmaxf(big, (float)v[j][k]);
           if (big > m) {                           // (rescaled by the difference of the ROUNDED products that the terms are shifted by)
             const float to = rounded(big * c);
             s = m == -__builtin_inff() ? s : s * __builtin_amdgcn_exp2f(own_mc - to);
@@ -144,7 +158,10 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_distill_rows(DistillA
             own_mc = to;
           }
 #pragma unroll
-          for (int k = 0; k < VE; ++k) s += __builtin_amdgcn_exp2f(fmaf((float)v[k], c, -own_mc));
+          for (int j = 0; j < 4; ++j)
+            if (at + j * TPR * VE < a.vocab)
+#pragma unroll
+              for (int k = 0; k < VE; ++k) s += __builtin_amdgcn_exp2f(fmaf((float)v[j][k], c, -own_mc));
         }
       }
     }
@@ -188,12 +205,20 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_distill_rows(DistillA
           store_pack<ODD>(g + at, left, o);
         }
       } else {
-        for (int at = t * VE; at < a.vocab; at += TPR * VE) {
-          const V v = load_pack<ODD>(z + at, a.vocab - at);
-          V o;
+        for (int at = t * VE; at < a.vocab; at += 4 * TPR * VE) {
+          V v[4];
 #pragma unroll
-          for (int k = 0; k < VE; ++k) o[k] = (T)(__builtin_amdgcn_exp2f(fmaf((float)v[k], c, -mc)) * kq);
-          store_pack<ODD>(g + at, a.vocab - at, o);
+          for (int j = 0; j < 4; ++j)
+            if (at + j * TPR * VE < a.vocab) v[j] = load_pack<ODD>(z + at + j * TPR * VE, a.vocab - at - j * TPR * VE);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int left = a.vocab - at - j * TPR * VE;
+            if (left <= 0) continue;
+            V o;
+#pragma unroll
+            for (int k = 0; k < VE; ++k) o[k] = (T)(__builtin_amdgcn_exp2f(fmaf((float)v[j][k], c, -mc)) * kq);
+            store_pack<ODD>(g + at + j * TPR * VE, left, o);
+          }
         }
       }
     }
@@ -210,7 +235,7 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_distill_rows(DistillA
         for (int k = t; k < K; k += SL) {
           const int id = sid[k];
           if (id < 0) continue;
-          const float lp = st[k] - ls, p = __builtin_amdgcn_exp2f(lp), zk = fmaf((float)z[id], c, -mc);
+          const float lp = st[k] - ls, p = __builtin_amdgcn_exp2f(lp), zk = fmaf(sz[k], c, -mc);
           if (!(p == 0.f)) part = fmaf(p, lp - (zk - lq), part);
           if (!a.g || k1 == 0.f) continue;
           float sum = 0.f;                         // p of every slot with this id; only the first of them writes
@@ -246,23 +271,48 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_distill_rows(DistillA
   }
 }
 
-// A lane a row, up to VM entries in registers; the first KR slots too.
+// A lane a row, up to VM entries in registers; the first KR slots too.  Rows that lie side by side go through LDS, 64 of a wave at a time
+// in whole lines (a lane's own 16-byte pieces of a row of 48 bytes touch every line three times, and store parts of lines).
 template <typename T, int VM>
 __global__ __launch_bounds__(256) void k_distill_lanes(DistillArgs a) {
   constexpr int VE = Pack<T>::n, NP = VM / VE, KR = 8;
   typedef typename Pack<T>::V V;
-  __shared__ float wave_sum[4];
+  constexpr int PITCH = VM + 1;
+  __shared__ float wave_sum[4], staged[4][64 * PITCH];
+  float* tile = staged[threadIdx.x >> 6];
+  const int lane = threadIdx.x & 63;
+  const unsigned by_vocab = ((1u << 20) + a.vocab - 1) / a.vocab;          // e / vocab = e * this >> 20 for e < 64 * 32
+  const bool in_dense = a.zs == a.vocab, out_dense = a.g && a.gs == a.vocab;
   if (a.skip_if_one && *a.up == 1.f) return;
   const float c = 1.44269504088896341f / a.temperature, base = factor_of(a);
   float total = 0.f;
-  for (long long row = (long long)blockIdx.x * 256 + threadIdx.x; row < a.rows; row += (long long)gridDim.x * 256) {
-    const float w = a.w ? a.w[row] : 1.f;
+  for (long long first = (long long)blockIdx.x * 256 + (threadIdx.x & ~63); first < a.rows; first += (long long)gridDim.x * 256) {
+    const bool act = first + lane < a.rows;
+    const long long row = act ? first + lane : a.rows - 1;        // (a lane beyond the last row repeats it and writes nothing)
+    const float w = !act ? 0.f : a.w ? a.w[row] : 1.f;
     const T* z = static_cast<const T*>(a.z) + row * a.zs;
+    const int held = (int)(a.rows - first < 64 ? a.rows - first : 64) * a.vocab;      // elements of this wave's rows
+    if (in_dense) {
+      for (int e = lane * VE; e < held; e += 64 * VE) {
+        const V v = load_pack<true>(static_cast<const T*>(a.z) + first * a.vocab + e, held - e);
+#pragma unroll
+        for (int k = 0; k < VE; ++k) {
+          const unsigned r = (unsigned)(e + k) * by_vocab >> 20;
+          if (e + k < held) tile[r * PITCH + (e + k) - r * a.vocab] = (float)v[k];
+        }
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+    }
     const int K = a.top, V_ = a.vocab;
     float x[VM], m = -__builtin_inff(), s = 0.f;
     int id[KR];
     float tv[KR], mt = -__builtin_inff();
     bool bad = false;
+    if (in_dense) {
+#pragma unroll
+      for (int k = 0; k < VM; ++k) x[k] = k < V_ ? tile[(int)(row - first) * PITCH + k] : -__builtin_inff();
+    } else
 #pragma unroll
     for (int j = 0; j < NP; ++j) {
       if (j * VE < V_) {
@@ -339,17 +389,31 @@ __global__ __launch_bounds__(256) void k_distill_lanes(DistillArgs a) {
     if (a.g) {
       T* g = static_cast<T*>(a.g) + row * a.gs;
 #pragma unroll
-      for (int j = 0; j < NP; ++j) {
-        if (j * VE >= V_) continue;
-        V o;
+      for (int k = 0; k < VM; ++k) {
+        const float v = k1 == 0.f ? 0.f : fmaf(__builtin_amdgcn_exp2f(x[k]), kq, -k1 * mass[k]);
+        if (k < V_ && act) {
+          if (out_dense) tile[lane * PITCH + k] = v;
+          else g[k] = (T)v;
+        }
+      }
+      if (out_dense) {
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        for (int e = lane * VE; e < held; e += 64 * VE) {
+          V o;
 #pragma unroll
-        for (int k = 0; k < VE; ++k)
-          o[k] = (T)(k1 == 0.f ? 0.f : fmaf(__builtin_amdgcn_exp2f(x[j * VE + k]), kq, -k1 * mass[j * VE + k]));
-        store_pack<true>(g + j * VE, V_ - j * VE, o);
+          for (int k = 0; k < VE; ++k) {
+            const unsigned r = (unsigned)(e + k) * by_vocab >> 20;
+            o[k] = (T)(e + k < held ? tile[r * PITCH + (e + k) - r * a.vocab] : 0.f);
+          }
+          store_pack<true>(static_cast<T*>(a.g) + first * a.vocab + e, held - e, o);
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
       }
     }
     const float loss = coef == 0.f ? 0.f : base * coef * a.temperature * a.temperature * kLn2 * part;
-    if (a.rows_out) a.rows_out[row] = loss;
+    if (a.rows_out && act) a.rows_out[row] = loss;
     total += loss;
   }
   if (a.sums) {
@@ -378,18 +442,19 @@ struct Geometry { int tpr, nv; };       // nv 0: the row is read twice
 template <typename T> Geometry geometry(int vocab, int top) {
   const long long packs = (vocab + Pack<T>::n - 1) / Pack<T>::n;
   int tpr = 8;
-  while (tpr < 64 && (packs > tpr || (256 / tpr) * 8 * top > 32768)) tpr *= 2;
+  while (tpr < 64 && (packs > tpr || (256 / tpr) * 12 * top > 32768)) tpr *= 2;
   if (packs <= tpr) return {tpr, 1};
   if (packs <= 64 * 4) return {64, 4};
   if (packs <= 256 * 4) return {256, 4};
   if (packs <= 256 * 8) return {256, 8};
-  if (packs <= 1024 * 4) return {1024, 4};
-  if (packs <= 1024 * 8) return {1024, 8};
+  if (packs <= 512 * 8) return {512, 8};
+  if (packs <= 512 * 16) return {512, 16};
+  if (packs <= 1024 * 16) return {1024, 16};
   return {1024, 0};
 }
 bool by_lanes(int vocab) { return vocab <= 32; }
 template <typename T> int blocks_of(long long rows, int vocab, int top) {
-  if (by_lanes(vocab)) return grid_for(rows, 256);
+  if (by_lanes(vocab)) return (int)(rows <= 16384 * 256 ? (rows + 255) / 256 : 16384);
   const int tpr = geometry<T>(vocab, top).tpr, tpb = tpr > 256 ? tpr : 256;
   const long long g = (rows + tpb / tpr - 1) / (tpb / tpr), most = (long long)kMaxBlocks * 256 / tpb;
   return (int)(g < most ? g : most);
@@ -403,7 +468,7 @@ template <typename T, bool ODD>
 void launch_rows(const DistillArgs& a, int blocks, hipStream_t st) {
   const Geometry g = geometry<T>(a.vocab, a.top);
   const int tpb = g.tpr > 256 ? g.tpr : 256;
-  const size_t lds = (size_t)(tpb / g.tpr) * 2 * a.top * sizeof(float);
+  const size_t lds = (size_t)(tpb / g.tpr) * 3 * a.top * sizeof(float);
 #define OMNIHD_DISTILL(R, N) hipLaunchKernelGGL((k_distill_rows<T, R, N, ODD>), dim3(blocks), dim3(tpb), lds, st, a)
   if (g.tpr == 8) OMNIHD_DISTILL(8, 1);
   else if (g.tpr == 16) OMNIHD_DISTILL(16, 1);
@@ -412,8 +477,9 @@ void launch_rows(const DistillArgs& a, int blocks, hipStream_t st) {
   else if (g.tpr == 64) OMNIHD_DISTILL(64, 4);
   else if (g.tpr == 256 && g.nv == 4) OMNIHD_DISTILL(256, 4);
   else if (g.tpr == 256) OMNIHD_DISTILL(256, 8);
-  else if (g.nv == 4) OMNIHD_DISTILL(1024, 4);
-  else if (g.nv == 8) OMNIHD_DISTILL(1024, 8);
+  else if (g.nv == 8) OMNIHD_DISTILL(512, 8);
+  else if (g.tpr == 512) OMNIHD_DISTILL(512, 16);
+  else if (g.nv == 16) OMNIHD_DISTILL(1024, 16);
   else OMNIHD_DISTILL(1024, 0);
 #undef OMNIHD_DISTILL
 }

@@ -116,12 +116,12 @@ PROTOTYPES = {
     "omnihd_iou_bev_matrix": (c_int, [c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p]),
     "omnihd_token_embed_fwd": (c_int, [c_void_p, c_int, c_longlong, c_void_p, c_int, c_longlong, c_longlong, c_int, c_float, c_void_p, c_int,
                     c_void_p]),
-    "omnihd_token_embed_bwd_workspace_bytes": (c_size_t, [c_longlong, c_int]),
+    "omnihd_token_embed_bwd_workspace_bytes": (c_size_t, [c_longlong, c_longlong, c_int]),
     "omnihd_token_embed_bwd": (c_int, [c_void_p, c_int, c_longlong, c_void_p, c_int, c_longlong, c_longlong, c_int, c_float, c_longlong, c_void_p,
                     c_int, c_void_p, c_size_t, c_void_p]),
     "omnihd_block_join_fwd": (c_int, [c_void_p, c_longlong, c_int, c_void_p, c_longlong, c_int, c_void_p, c_int, c_void_p, c_int, c_int, c_longlong,
                     c_longlong, c_void_p, c_int, c_float, c_float, c_longlong, c_int, c_void_p, c_void_p, c_void_p, c_void_p]),
-    "omnihd_block_join_bwd_workspace_bytes": (c_size_t, [c_longlong, c_int, c_int, c_longlong]),
+    "omnihd_block_join_bwd_workspace_bytes": (c_size_t, [c_longlong, c_int, c_int, c_longlong, c_int]),
     "omnihd_block_join_bwd": (c_int, [c_void_p, c_longlong, c_int, c_void_p, c_longlong, c_int, c_void_p, c_int, c_void_p, c_int, c_int, c_longlong,
                     c_longlong, c_void_p, c_int, c_float, c_longlong, c_int, c_void_p, c_void_p, c_longlong, c_void_p, c_longlong, c_void_p,
                     c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),

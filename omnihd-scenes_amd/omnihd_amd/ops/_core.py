@@ -148,5 +148,31 @@ def _rows2d(t, dim):
     return t.contiguous().view(-1, dim)
 
 
-def _pitch(rows):
-    return rows.stride(0) if rows.shape[0] > 1 else rows.shape[1]
+def _rows_of(t, dim):
+    """(address, pitch, what keeps the memory alive) of (..., dim) as rows; (None, 0, None) of None."""
+    if t is None:
+        return None, 0, None
+    if t.is_contiguous():
+        return t.data_ptr(), dim, t
+    v = _rows2d(t, dim)
+    return v.data_ptr(), v.stride(0) if v.shape[0] > 1 else dim, v
+
+
+def _dense_like(t):
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+
+
+def _no_second_order(what):
+    """In a backward pass: grad mode is on only where the gradients' own graph is wanted."""
+    if torch.is_grad_enabled():
+        raise RuntimeError(f"{what}: second derivatives (create_graph=True) are not supported")
+
+
+def _sized_workspace(key, size, dev):
+    """A workspace of its own, of the size that ``size()`` gives for `key` (asked for once)."""
+    n = _SIZE_CACHE.get(key)
+    if n is None:
+        if len(_SIZE_CACHE) > 4096:                       # ragged batches bring new sizes for ever
+            _SIZE_CACHE.clear()
+        n = _SIZE_CACHE[key] = max(int(size()), 256)
+    return torch.empty(n, dtype=torch.uint8, device=dev)

@@ -9,11 +9,11 @@ import weakref
 
 import numpy as np
 import torch
-from torch.autograd.function import once_differentiable
 
 from .._env import env as _env
 from .._lib import check, lib
-from ._core import (_TYPE_CODE, _on, _pitch, _ptr, _raw_stream, _rows2d, _same_device, _stream, _want, _want_rows, _workspace)
+from ._core import (_TYPE_CODE, _dense_like, _no_second_order, _on, _ptr, _raw_stream, _rows_of, _same_device, _sized_workspace, _stream,
+    _want, _want_rows, _workspace)
 
 
 
@@ -177,11 +177,12 @@ def anchor_loss(cls_score, bbox_pred, dir_pred, anchors, gt_boxes, gt_labels, gt
 # Token embedding: scaled row lookup, gradient by sorted tokens (csrc/token_embed.hip)
 # --------------------------------------------------------------------------------------------
 def _embed_forward(ids, table, scale, out_dtype):
-    out = torch.empty(ids.shape + (table.shape[1],), dtype=out_dtype, device=table.device)
+    vocab, dim = table.shape
+    out = torch.empty(ids.shape + (dim,), dtype=out_dtype, device=table.device)
     if out.numel():
         with _on(table.device):
-            check(lib().omnihd_token_embed_fwd(ids.data_ptr(), int(ids.dtype == torch.int64), ids.numel(), table.data_ptr(), _TYPE_CODE[table.dtype],
-                                               _pitch(table), table.shape[0], table.shape[1], scale, out.data_ptr(), _TYPE_CODE[out_dtype],
+            check(lib().omnihd_token_embed_fwd(ids.data_ptr(), ids.dtype == torch.int64, ids.numel(), table.data_ptr(), _TYPE_CODE[table.dtype],
+                                               table.stride(0) if vocab > 1 else dim, vocab, dim, scale, out.data_ptr(), _TYPE_CODE[out_dtype],
                                                _raw_stream()), "omnihd_token_embed_fwd")
     return out
 
@@ -190,23 +191,22 @@ class _TokenEmbed(torch.autograd.Function):
     @staticmethod
     def forward(ctx, table, ids, scale, padding, out_dtype):
         ctx.save_for_backward(ids)
-        ctx.meta = (tuple(table.shape), table.dtype, scale, padding)
+        ctx.meta = (table.shape, table.dtype, scale, padding)
         return _embed_forward(ids, table, scale, out_dtype)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, g):
+        _no_second_order("token_embedding")
         ids, = ctx.saved_tensors
-        (vocab, dim), dtype, scale, padding = ctx.meta
-        dev = g.device
-        g2 = _rows2d(g, dim)
-        grad = torch.empty((vocab, dim), dtype=dtype, device=dev)
-        L, n = lib(), ids.numel()
+        shape, dtype, scale, padding = ctx.meta
+        vocab, dim = shape
+        dev, n, L = g.device, ids.numel(), lib()
+        gp, gs, keep = _rows_of(g, dim)
+        grad = torch.empty(shape, dtype=dtype, device=dev)
         with _on(dev):
-            ws = _workspace(L.omnihd_token_embed_bwd_workspace_bytes(n, dim), dev)
-            check(L.omnihd_token_embed_bwd(ids.data_ptr(), int(ids.dtype == torch.int64), n, g2.data_ptr(), _TYPE_CODE[g2.dtype], _pitch(g2), vocab, dim,
-                                           scale, padding, grad.data_ptr(), _TYPE_CODE[dtype], ws.data_ptr(), ws.numel(), _raw_stream()),
-                  "omnihd_token_embed_bwd")
+            ws = _sized_workspace(("embed", n, vocab, dim), lambda: L.omnihd_token_embed_bwd_workspace_bytes(n, vocab, dim), dev)
+            check(L.omnihd_token_embed_bwd(ids.data_ptr(), ids.dtype == torch.int64, n, gp, _TYPE_CODE[g.dtype], gs, vocab, dim, scale, padding,
+                                           grad.data_ptr(), _TYPE_CODE[dtype], ws.data_ptr(), ws.numel(), _raw_stream()), "omnihd_token_embed_bwd")
         return grad, None, None, None, None
 
 
@@ -246,20 +246,26 @@ _DISTILL_MAX_TOP = 256
 def _distill_call(z, t, ids, weight, avg, meta, grad=None, up=None, skip_if_one=False, want_loss=True):
     """One launch over the rows: the loss (one number, or one a row) and / or the gradient into `grad`."""
     temperature, factor, per_row = meta
-    vocab, top = z.shape[-1], t.shape[-1]
-    rows, dev = z.numel() // vocab, z.device
-    z2, t2, i2 = _rows2d(z, vocab), _rows2d(t, top), _rows2d(ids, top)
-    loss = torch.empty(z.shape[:-1] if per_row else (), dtype=torch.float32, device=dev) if want_loss else None
+    vocab, top, dev = z.shape[-1], t.shape[-1], z.device
+    rows, zt = z.numel() // vocab, _TYPE_CODE[z.dtype]
+    zp, zs, keep_z = _rows_of(z, vocab)
+    tp, ts, keep_t = _rows_of(t, top)
+    ip, ist, keep_i = _rows_of(ids, top)
+    loss = row_loss = ws = None
     L = lib()
     with _on(dev):
-        ws = _workspace(L.omnihd_topk_distill_workspace_bytes(rows, vocab, top, _TYPE_CODE[z.dtype]), dev) if want_loss and not per_row else None
-        check(L.omnihd_topk_distill(z2.data_ptr(), _TYPE_CODE[z.dtype], _pitch(z2), t2.data_ptr(), _TYPE_CODE[t.dtype], _pitch(t2), i2.data_ptr(),
-                                    int(ids.dtype == torch.int64), _pitch(i2), None if weight is None else weight.data_ptr(), rows, vocab, top,
-                                    temperature, factor, None if avg is None else avg.data_ptr(), None if up is None else up.data_ptr(),
-                                    int(up is not None and per_row), int(skip_if_one), None if grad is None else grad.data_ptr(), vocab,
-                                    loss.data_ptr() if want_loss and per_row else None, loss.data_ptr() if want_loss and not per_row else None,
+        if want_loss:
+            if per_row:
+                row_loss = torch.empty(z.shape[:-1], dtype=torch.float32, device=dev)
+            else:
+                loss = torch.empty((), dtype=torch.float32, device=dev)
+                ws = _sized_workspace(("distill", rows, vocab, top, zt), lambda: L.omnihd_topk_distill_workspace_bytes(rows, vocab, top, zt), dev)
+        check(L.omnihd_topk_distill(zp, zt, zs, tp, _TYPE_CODE[t.dtype], ts, ip, ids.dtype == torch.int64, ist, None if weight is None else weight.data_ptr(),
+                                    rows, vocab, top, temperature, factor, None if avg is None else avg.data_ptr(), None if up is None else up.data_ptr(),
+                                    up is not None and per_row, skip_if_one, None if grad is None else grad.data_ptr(), vocab,
+                                    None if row_loss is None else row_loss.data_ptr(), None if loss is None else loss.data_ptr(),
                                     None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(), _raw_stream()), "omnihd_topk_distill")
-    return loss
+    return row_loss if per_row else loss
 
 
 class _TopkDistill(torch.autograd.Function):
@@ -273,22 +279,22 @@ class _TopkDistill(torch.autograd.Function):
         ctx.meta, ctx.fresh = meta, False
         grad = None
         if not meta[2] and not torch.cuda.is_current_stream_capturing():
-            grad = torch.empty(z.shape, dtype=z.dtype, device=z.device)
+            grad = _dense_like(z)
             ctx.fresh = True
         loss = _distill_call(z, t, ids, weight, avg, meta, grad)
         ctx.save_for_backward(z, t, ids, weight, avg, grad)
         return loss
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, up):
+        _no_second_order("topk_distill_loss")
         z, t, ids, weight, avg, grad = ctx.saved_tensors
-        up = up.to(torch.float32).contiguous()
+        up = up.contiguous()                               # (fp32, as the loss is)
         in_place = ctx.fresh and not torch.cuda.is_current_stream_capturing()
         if in_place:
             ctx.fresh = False
         else:
-            grad = torch.empty(z.shape, dtype=z.dtype, device=z.device)
+            grad = _dense_like(z)
         _distill_call(z, t, ids, weight, avg, ctx.meta, grad, up, skip_if_one=in_place, want_loss=False)
         return grad, None, None, None, None, None
 

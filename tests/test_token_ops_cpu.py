@@ -103,8 +103,8 @@ def test_c_entries_refuse_before_any_launch():
         args[at] = bad
         assert L.omnihd_token_embed_fwd(*args) == ARG, (at, bad)
         assert L.omnihd_last_error()
-    need = L.omnihd_token_embed_bwd_workspace_bytes(5, 8)
-    back = [p, 1, 5, p, 0, 8, 4, 8, 1.0, -1, p, 0, p, need, None]
+    need = L.omnihd_token_embed_bwd_workspace_bytes(5, 7, 8)
+    back = [p, 1, 5, p, 0, 8, 7, 8, 1.0, -1, p, 0, p, need, None]
     for at, bad, status in ((13, need - 1, WORKSPACE), (12, None, ARG), (10, None, ARG), (3, None, ARG), (5, 7, ARG), (2, -1, ARG)):
         args = list(back)
         args[at] = bad
@@ -114,7 +114,7 @@ def test_c_entries_refuse_before_any_launch():
         args = list(fwd)
         args[at] = bad
         assert L.omnihd_block_join_fwd(*args) == ARG, (at, bad)
-    need = L.omnihd_block_join_bwd_workspace_bytes(5, 8, 1, 5)
+    need = L.omnihd_block_join_bwd_workspace_bytes(5, 8, 1, 5, 1)
     back = [p, 8, 0, p, 8, 0, p, 0, p, 0, 1, 8, 5, p, 0, 1.0, 5, 8, p, p, 8, p, 8, p, p, p, p, p, p, need, None]
     for at, bad, status in ((29, need - 1, WORKSPACE), (28, None, ARG), (18, None, ARG), (0, None, ARG), (6, None, ARG), (13, None, ARG), (3, None, ARG), (17, 20000, ARG)):
         args = list(back)
@@ -132,7 +132,7 @@ def test_c_entries_refuse_before_any_launch():
 def test_workspaces_cover_long_inputs():
     from omnihd_amd._lib import lib
     L = lib()
-    assert L.omnihd_token_embed_bwd_workspace_bytes(0, 8) > 0
-    assert L.omnihd_token_embed_bwd_workspace_bytes((1 << 31) - 1, 64) > 2 * 4 * ((1 << 31) - 1)
+    assert L.omnihd_token_embed_bwd_workspace_bytes(0, 9, 8) > 0
+    assert L.omnihd_token_embed_bwd_workspace_bytes((1 << 31) - 1, 32000, 64) > 2 * 4 * ((1 << 31) - 1)
     assert L.omnihd_topk_distill_workspace_bytes(0, 8, 1, 0) > 0 and L.omnihd_topk_distill_workspace_bytes(5, 8, 300, 0) == 0
-    assert L.omnihd_block_join_bwd_workspace_bytes(0, 8, 0, 1) > 0
+    assert L.omnihd_block_join_bwd_workspace_bytes(0, 8, 0, 1, 1) > 0

@@ -248,3 +248,13 @@ def test_stream_and_graph(cuda):
         torch.cuda.synchronize()
         loss, grad = step()
         assert torch.equal(loss, loss_g) and torch.equal(grad, grad_g), k
+
+
+def test_second_derivatives_are_refused(cuda):
+    from omnihd_amd import ops
+    z, t, ids, _ = inputs(5, 40, 3, F, F, 1)
+    z.requires_grad_()
+    w = torch.ones(40, device="cuda").requires_grad_()
+    for value in (ops.topk_distill_loss(z, t, ids), ops.block_norm(z, w).sum(), ops.block_join(z, z, next_weight=w)[1].sum(), ops.token_embedding(ids, z).sum()):
+        with pytest.raises(RuntimeError, match="second derivatives"):
+            torch.autograd.grad(value, z, create_graph=True)
