@@ -131,7 +131,10 @@ PROTOTYPES = {
                     c_void_p]),
 }
 
+_TORCH_PATH = os.path.join(os.path.dirname(_HERE), "lib", "omnihd_torch.so")
+
 _lib = None
+_torch_ops = None
 
 
 def library_path():
@@ -153,6 +156,25 @@ def lib():
             fn.argtypes = args
         _lib = handle
     return _lib
+
+
+def torch_ops():
+    """Load (once) the torch face of the token operators (csrc/torch_tokens.cpp); it calls the entries of the library that ``lib()`` loads."""
+    global _torch_ops
+    if _torch_ops is None:
+        import importlib.machinery
+        import importlib.util
+
+        import torch  # noqa: F401  (its libraries have to be loaded first)
+        if not os.path.exists(_TORCH_PATH):
+            raise RuntimeError(f"{_TORCH_PATH} is missing: build it with `make -C omnihd-scenes_amd/csrc` (or __graft_entry__.build())")
+        loader = importlib.machinery.ExtensionFileLoader("omnihd_torch", _TORCH_PATH)
+        module = importlib.util.module_from_spec(importlib.util.spec_from_loader("omnihd_torch", loader))
+        loader.exec_module(module)
+        handle = lib()
+        module.bind({name: ctypes.cast(getattr(handle, name), c_void_p).value for name in PROTOTYPES})
+        _torch_ops = module
+    return _torch_ops
 
 
 def require_gpu():

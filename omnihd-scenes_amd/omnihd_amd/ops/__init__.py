@@ -18,7 +18,7 @@ replace functions through it); state that code REBINDS lives in one part and is 
 from . import _core
 from ._core import (_ptr, _current_device, _raw_stream, _stream, _want, _same_device, _workspace, _NULL_CTX, _SIZE_CACHE, _on,
     _WGRAD_WS, _wgrad_workspace, _want_cl, _pair_same, deterministic, FAST_PATHS, _CL, _rows_view, _f32c,
-    _TYPE_CODE, _want_rows, _rows2d, _rows_of, _dense_like, _no_second_order, _sized_workspace)
+    _ROW_TYPES, _want_rows)
 from . import pool
 from .pool import (bev_pool_v2_forward, bev_pool_v2_backward, bev_pool_v2_forward_csr, _PREFETCH_STREAMS, prefetch,
     bev_pool_v2_forward_direct, bev_pool_v2_backward_patch, tile_descriptors, csr_tiles, _nhwc_rows, _DepthHead,
@@ -60,9 +60,9 @@ from .conv_bf16 import (_ConvBiasColsum, wgrad_split_padded, conv_bias_colsum_su
     deconv_split, deconv_supported, deconv_hip_wgrad)
 from . import norm
 from .norm import (_AffineAct, affine_act_supported, affine_act, _BnTrainAct, bn_train_supported, bn_train_act, _BLOCK_MAX_DIM, _GATE_NONE, _GATE_ROWS,
-    _GATE_TOKEN, _GATE_FULL, _gate_layout, _block_args, _BlockJoin, _block_forward, _block_checks, block_norm, block_join)
+    _GATE_TOKEN, _GATE_FULL, _gate_layout, _block_checks, block_norm, block_join)
 from . import misc
 from .misc import (_DcnSample, dcn3x3_sample, dcn3x3_supported, nms_rotated, iou_bev_matrix, _AnchorLoss, anchor_loss,
-    _embed_forward, _TokenEmbed, token_embedding, _DISTILL_MAX_TOP, _distill_call, _TopkDistill, topk_distill_loss)
+    token_embedding, _DISTILL_MAX_TOP, topk_distill_loss)
 
 PARTS = (_core, pool, radar, conv_kernels, policy, planes, weights, streams, conv_fp32, conv_bf16, norm, misc)

@@ -124,55 +124,11 @@ def _f32c(t):
 # --------------------------------------------------------------------------------------------
 # Token rows (norms of a residual stream, embedding, distillation)
 # --------------------------------------------------------------------------------------------
-_TYPE_CODE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}       # include/omnihd_hip.h: element type codes
+_ROW_TYPES = (torch.float32, torch.bfloat16, torch.float16)
 
 
 def _want_rows(t, name):
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise RuntimeError(f"{name} must be a CUDA(HIP) tensor; the HIP ops have no CPU path")
-    if t.dtype not in _TYPE_CODE:
+    if t.dtype not in _ROW_TYPES:
         raise TypeError(f"{name} must be float32, bfloat16 or float16, got {t.dtype}")
-
-
-def _rows2d(t, dim):
-    """(..., dim) as rows with one pitch between them: a view where the strides allow it, else a copy."""
-    if t.is_contiguous():
-        return t.view(-1, dim)
-    if dim == 1 or t.stride(-1) == 1:
-        try:
-            v = t.view(-1, dim)
-        except RuntimeError:
-            v = None
-        if v is not None and (v.shape[0] <= 1 or v.stride(0) >= dim):
-            return v
-    return t.contiguous().view(-1, dim)
-
-
-def _rows_of(t, dim):
-    """(address, pitch, what keeps the memory alive) of (..., dim) as rows; (None, 0, None) of None."""
-    if t is None:
-        return None, 0, None
-    if t.is_contiguous():
-        return t.data_ptr(), dim, t
-    v = _rows2d(t, dim)
-    return v.data_ptr(), v.stride(0) if v.shape[0] > 1 else dim, v
-
-
-def _dense_like(t):
-    return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
-
-
-def _no_second_order(what):
-    """In a backward pass: grad mode is on only where the gradients' own graph is wanted."""
-    if torch.is_grad_enabled():
-        raise RuntimeError(f"{what}: second derivatives (create_graph=True) are not supported")
-
-
-def _sized_workspace(key, size, dev):
-    """A workspace of its own, of the size that ``size()`` gives for `key` (asked for once)."""
-    n = _SIZE_CACHE.get(key)
-    if n is None:
-        if len(_SIZE_CACHE) > 4096:                       # ragged batches bring new sizes for ever
-            _SIZE_CACHE.clear()
-        n = _SIZE_CACHE[key] = max(int(size()), 256)
-    return torch.empty(n, dtype=torch.uint8, device=dev)

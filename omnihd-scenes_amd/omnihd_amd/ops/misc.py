@@ -11,9 +11,8 @@ import numpy as np
 import torch
 
 from .._env import env as _env
-from .._lib import check, lib
-from ._core import (_TYPE_CODE, _dense_like, _no_second_order, _on, _ptr, _raw_stream, _rows_of, _same_device, _sized_workspace, _stream,
-    _want, _want_rows, _workspace)
+from .._lib import check, lib, torch_ops
+from ._core import _ROW_TYPES, _on, _ptr, _raw_stream, _same_device, _stream, _want, _want_rows, _workspace
 
 
 
@@ -176,40 +175,6 @@ def anchor_loss(cls_score, bbox_pred, dir_pred, anchors, gt_boxes, gt_labels, gt
 # --------------------------------------------------------------------------------------------
 # Token embedding: scaled row lookup, gradient by sorted tokens (csrc/token_embed.hip)
 # --------------------------------------------------------------------------------------------
-def _embed_forward(ids, table, scale, out_dtype):
-    vocab, dim = table.shape
-    out = torch.empty(ids.shape + (dim,), dtype=out_dtype, device=table.device)
-    if out.numel():
-        with _on(table.device):
-            check(lib().omnihd_token_embed_fwd(ids.data_ptr(), ids.dtype == torch.int64, ids.numel(), table.data_ptr(), _TYPE_CODE[table.dtype],
-                                               table.stride(0) if vocab > 1 else dim, vocab, dim, scale, out.data_ptr(), _TYPE_CODE[out_dtype],
-                                               _raw_stream()), "omnihd_token_embed_fwd")
-    return out
-
-
-class _TokenEmbed(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, table, ids, scale, padding, out_dtype):
-        ctx.save_for_backward(ids)
-        ctx.meta = (table.shape, table.dtype, scale, padding)
-        return _embed_forward(ids, table, scale, out_dtype)
-
-    @staticmethod
-    def backward(ctx, g):
-        _no_second_order("token_embedding")
-        ids, = ctx.saved_tensors
-        shape, dtype, scale, padding = ctx.meta
-        vocab, dim = shape
-        dev, n, L = g.device, ids.numel(), lib()
-        gp, gs, keep = _rows_of(g, dim)
-        grad = torch.empty(shape, dtype=dtype, device=dev)
-        with _on(dev):
-            ws = _sized_workspace(("embed", n, vocab, dim), lambda: L.omnihd_token_embed_bwd_workspace_bytes(n, vocab, dim), dev)
-            check(L.omnihd_token_embed_bwd(ids.data_ptr(), ids.dtype == torch.int64, n, gp, _TYPE_CODE[g.dtype], gs, vocab, dim, scale, padding,
-                                           grad.data_ptr(), _TYPE_CODE[dtype], ws.data_ptr(), ws.numel(), _raw_stream()), "omnihd_token_embed_bwd")
-        return grad, None, None, None, None
-
-
 def token_embedding(ids, table, scale=1.0, padding_idx=None, out_dtype=None):
     """``scale * table[ids]``: ids of any shape, int64 or int32; table (vocab, D) fp32, bf16 or fp16 with dense rows (a row pitch is fine).
     ``out_dtype``: the table's type (the default), or a 16-bit type for an fp32 table.  An id outside [0, vocab) gives a row of NaN.
@@ -224,79 +189,20 @@ def token_embedding(ids, table, scale=1.0, padding_idx=None, out_dtype=None):
         raise TypeError("ids must be an int64 or int32 tensor")
     _same_device(table, ids)
     out_dtype = table.dtype if out_dtype is None else out_dtype
-    if out_dtype not in _TYPE_CODE or (out_dtype != table.dtype and table.dtype != torch.float32):
+    if out_dtype not in _ROW_TYPES or (out_dtype != table.dtype and table.dtype != torch.float32):
         raise TypeError(f"out_dtype {out_dtype} of a {table.dtype} table: wanted the table's type, or a 16-bit type for an fp32 table")
     padding = -1
     if padding_idx is not None:
         if not -table.shape[0] <= padding_idx < table.shape[0]:
             raise ValueError(f"padding_idx {padding_idx} is not a row of a table of {table.shape[0]}")
         padding = int(padding_idx) % table.shape[0]
-    ids = ids.contiguous()
-    if torch.is_grad_enabled() and table.requires_grad:
-        return _TokenEmbed.apply(table, ids, float(scale), padding, out_dtype)
-    return _embed_forward(ids, table, float(scale), out_dtype)
+    return torch_ops().token_embedding(ids, table, scale, padding, out_dtype)
 
 
 # --------------------------------------------------------------------------------------------
 # Distillation from a teacher's top logits (csrc/topk_distill.hip)
 # --------------------------------------------------------------------------------------------
 _DISTILL_MAX_TOP = 256
-
-
-def _distill_call(z, t, ids, weight, avg, meta, grad=None, up=None, skip_if_one=False, want_loss=True):
-    """One launch over the rows: the loss (one number, or one a row) and / or the gradient into `grad`."""
-    temperature, factor, per_row = meta
-    vocab, top, dev = z.shape[-1], t.shape[-1], z.device
-    rows, zt = z.numel() // vocab, _TYPE_CODE[z.dtype]
-    zp, zs, keep_z = _rows_of(z, vocab)
-    tp, ts, keep_t = _rows_of(t, top)
-    ip, ist, keep_i = _rows_of(ids, top)
-    loss = row_loss = ws = None
-    L = lib()
-    with _on(dev):
-        if want_loss:
-            if per_row:
-                row_loss = torch.empty(z.shape[:-1], dtype=torch.float32, device=dev)
-            else:
-                loss = torch.empty((), dtype=torch.float32, device=dev)
-                ws = _sized_workspace(("distill", rows, vocab, top, zt), lambda: L.omnihd_topk_distill_workspace_bytes(rows, vocab, top, zt), dev)
-        check(L.omnihd_topk_distill(zp, zt, zs, tp, _TYPE_CODE[t.dtype], ts, ip, ids.dtype == torch.int64, ist, None if weight is None else weight.data_ptr(),
-                                    rows, vocab, top, temperature, factor, None if avg is None else avg.data_ptr(), None if up is None else up.data_ptr(),
-                                    up is not None and per_row, skip_if_one, None if grad is None else grad.data_ptr(), vocab,
-                                    None if row_loss is None else row_loss.data_ptr(), None if loss is None else loss.data_ptr(),
-                                    None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(), _raw_stream()), "omnihd_topk_distill")
-    return row_loss if per_row else loss
-
-
-class _TopkDistill(torch.autograd.Function):
-    """The forward of a summed loss writes the logits' gradient too, while the row is in registers; the backward returns it, after a launch
-    that writes it again where the gradient arriving at the loss is not 1.  That second form alone (two passes instead of one and a half)
-    serves per-row losses, whose upstream gradient is not known in the forward, stream capture, whose replays may be of the backward
-    alone, and every further backward pass over the same forward."""
-
-    @staticmethod
-    def forward(ctx, z, t, ids, weight, avg, meta):
-        ctx.meta, ctx.fresh = meta, False
-        grad = None
-        if not meta[2] and not torch.cuda.is_current_stream_capturing():
-            grad = _dense_like(z)
-            ctx.fresh = True
-        loss = _distill_call(z, t, ids, weight, avg, meta, grad)
-        ctx.save_for_backward(z, t, ids, weight, avg, grad)
-        return loss
-
-    @staticmethod
-    def backward(ctx, up):
-        _no_second_order("topk_distill_loss")
-        z, t, ids, weight, avg, grad = ctx.saved_tensors
-        up = up.contiguous()                               # (fp32, as the loss is)
-        in_place = ctx.fresh and not torch.cuda.is_current_stream_capturing()
-        if in_place:
-            ctx.fresh = False
-        else:
-            grad = _dense_like(z)
-        _distill_call(z, t, ids, weight, avg, ctx.meta, grad, up, skip_if_one=in_place, want_loss=False)
-        return grad, None, None, None, None, None
 
 
 def topk_distill_loss(logits, teacher_logits, teacher_ids, temperature=1.0, row_weight=None, reduction="mean", avg_factor=None,
@@ -345,8 +251,4 @@ def topk_distill_loss(logits, teacher_logits, teacher_ids, temperature=1.0, row_
             raise ValueError(f"row_weight must be a tensor of shape {lead}")
         row_weight = row_weight.detach().to(torch.float32).contiguous()
     _same_device(logits, teacher_logits, teacher_ids, row_weight, avg)
-    meta = (temperature, factor, reduction == "none")
-    teacher_logits = teacher_logits.detach()
-    if torch.is_grad_enabled() and logits.requires_grad:
-        return _TopkDistill.apply(logits, teacher_logits, teacher_ids, row_weight, avg, meta)
-    return _distill_call(logits, teacher_logits, teacher_ids, row_weight, avg, meta)
+    return torch_ops().topk_distill(logits, teacher_logits, teacher_ids, row_weight, avg, temperature, factor, reduction == "none")

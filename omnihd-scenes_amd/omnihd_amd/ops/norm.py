@@ -11,9 +11,9 @@ import numpy as np
 import torch
 
 from .._env import env as _env
-from .._lib import check, lib
-from ._core import (FAST_PATHS, _SIZE_CACHE, _TYPE_CODE, _dense_like, _f32c, _no_second_order, _on, _raw_stream, _rows_of, _rows_view, _same_device,
-    _sized_workspace, _want, _want_rows, _wgrad_workspace)
+from .._lib import check, lib, torch_ops
+from ._core import (FAST_PATHS, _ROW_TYPES, _SIZE_CACHE, _f32c, _on, _raw_stream, _rows_view, _same_device, _want, _want_rows,
+    _wgrad_workspace)
 from .policy import _fp32_policy, f16_handover
 from .planes import _alloc_planes, _amax_slot, half_wanted, planes_wanted, tag_half, tag_planes, tag_producer
 
@@ -287,75 +287,6 @@ def _gate_layout(gate, shape):
                      f"and D, (..., 1), or the rows' own shape")
 
 
-def _block_args(x, y, post, gate, nxt, meta):
-    """The leading arguments that the forward and the backward share, and what keeps their memory alive."""
-    _scale, _eps, kind, per_gate, dim, act = meta
-    xp, xs, x2 = _rows_of(x, dim)
-    yp, ys, y2 = _rows_of(y, dim)
-    if post is not None:
-        post = post.contiguous()
-    if nxt is not None:
-        nxt = nxt.contiguous()
-    if kind == _GATE_TOKEN:
-        g2 = gate.contiguous()
-        gp, gs = g2.data_ptr(), 0
-    else:
-        gp, gs, g2 = _rows_of(gate, dim)
-    code = _TYPE_CODE
-    return ((xp, xs, code[x.dtype], yp, ys, code[act], None if post is None else post.data_ptr(), 0 if post is None else code[post.dtype], gp,
-             0 if gate is None else code[gate.dtype], kind, gs, per_gate, None if nxt is None else nxt.data_ptr(), 0 if nxt is None else code[nxt.dtype]),
-            (x2, y2, post, g2, nxt))
-
-
-class _BlockJoin(torch.autograd.Function):
-    """(x, y, post, gate, next) -> (x_out, h); y None: h = norm(x; next) alone.  See include/omnihd_hip.h: omnihd_block_join_fwd."""
-
-    @staticmethod
-    def forward(ctx, x, y, post, gate, nxt, meta):
-        out, h, stats = _block_forward(x, y, post, gate, nxt, meta, True)
-        ctx.save_for_backward(x, y, post, gate, nxt, stats)
-        ctx.meta = meta
-        ctx.set_materialize_grads(False)
-        return out, h
-
-    @staticmethod
-    def backward(ctx, d_out, d_h):
-        _no_second_order("block_join")
-        if d_out is None and d_h is None:
-            return None, None, None, None, None, None
-        x, y, post, gate, nxt, stats = ctx.saved_tensors
-        meta = ctx.meta
-        scale, _eps, kind, per_gate, dim, _act = meta
-        grads = [_dense_like(t) if want else None for t, want in zip((x, y, post, gate, nxt), ctx.needs_input_grad)]
-        rows, dev = stats.shape[0], x.device
-        if rows == 0:
-            return *(None if g is None else g.zero_() for g in grads), None
-        args, keep = _block_args(x, y, post, gate, nxt, meta)
-        dop, dos, keep_o = _rows_of(d_out, dim)
-        dhp, dhs, keep_h = _rows_of(d_h, dim)
-        L = lib()
-        with _on(dev):
-            ws = _sized_workspace(("block", rows, dim, kind, per_gate, y is None),
-                                  lambda: L.omnihd_block_join_bwd_workspace_bytes(rows, dim, kind, per_gate, int(y is not None)), dev)
-            check(L.omnihd_block_join_bwd(*args, scale, rows, dim, stats.data_ptr(), dop, dos, dhp, dhs, *[None if g is None else g.data_ptr() for g in grads],
-                                          ws.data_ptr(), ws.numel(), _raw_stream()), "omnihd_block_join_bwd")
-        return *grads, None
-
-
-def _block_forward(x, y, post, gate, nxt, meta, keep_stats):
-    scale, eps, _kind, _per_gate, dim, act = meta
-    dev, rows = x.device, x.numel() // dim
-    out = None if y is None else _dense_like(x)
-    h = None if nxt is None else torch.empty(x.shape, dtype=act, device=dev)
-    stats = torch.empty((rows, 2), dtype=torch.float32, device=dev) if keep_stats else None
-    if rows:
-        args, keep = _block_args(x, y, post, gate, nxt, meta)
-        with _on(dev):
-            check(lib().omnihd_block_join_fwd(*args, scale, eps, rows, dim, None if out is None else out.data_ptr(), None if h is None else h.data_ptr(),
-                                              None if stats is None else stats.data_ptr(), _raw_stream()), "omnihd_block_join_fwd")
-    return out, h, stats
-
-
 def _block_checks(x, eps, *weights):
     _want_rows(x, "x")
     if not 1 <= x.shape[-1] <= _BLOCK_MAX_DIM:
@@ -378,12 +309,9 @@ def block_norm(x, weight, eps=1e-6, out_dtype=None):
     if weight is None:
         raise TypeError("weight must be a tensor")
     act = x.dtype if out_dtype is None else out_dtype
-    if act not in _TYPE_CODE or (act != x.dtype and x.dtype != torch.float32):
+    if act not in _ROW_TYPES or (act != x.dtype and x.dtype != torch.float32):
         raise TypeError(f"out_dtype {act} with {x.dtype} rows: wanted the rows' type, or a 16-bit type for fp32 rows")
-    meta = (1.0, float(eps), _GATE_NONE, 1, x.shape[-1], act)
-    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
-        return _BlockJoin.apply(x, None, None, None, weight, meta)[1]
-    return _block_forward(x, None, None, None, weight, meta, False)[1]
+    return torch_ops().block_join(x, None, None, None, weight, 1.0, eps, _GATE_NONE, 1, act)[0]
 
 
 def block_join(x, y, post_weight=None, gate=None, residual_scale=1.0, next_weight=None, eps=1e-6):
@@ -407,9 +335,5 @@ def block_join(x, y, post_weight=None, gate=None, residual_scale=1.0, next_weigh
     if gate is not None:
         _want_rows(gate, "gate")
         kind, per_gate = _gate_layout(gate, tuple(x.shape))
-    meta = (float(residual_scale), float(eps), kind, per_gate, x.shape[-1], y.dtype)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, y, post_weight, gate, next_weight)):
-        out, h = _BlockJoin.apply(x, y, post_weight, gate, next_weight, meta)
-    else:
-        out, h, _ = _block_forward(x, y, post_weight, gate, next_weight, meta, False)
-    return out if next_weight is None else (out, h)
+    got = torch_ops().block_join(x, y, post_weight, gate, next_weight, residual_scale, eps, kind, per_gate, y.dtype)
+    return got[0] if next_weight is None else tuple(got)

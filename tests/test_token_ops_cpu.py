@@ -22,8 +22,8 @@ def ops(monkeypatch):
 
     def never():
         raise AssertionError("the library was reached")
-    monkeypatch.setattr(misc, "lib", never)
-    monkeypatch.setattr(norm, "lib", never)
+    monkeypatch.setattr(misc, "torch_ops", never)
+    monkeypatch.setattr(norm, "torch_ops", never)
     return ops
 
 
@@ -127,6 +127,15 @@ def test_c_entries_refuse_before_any_launch():
         args = list(call)
         args[at] = bad
         assert L.omnihd_topk_distill(*args) == status, (at, bad)
+
+
+def test_the_torch_face_loads_without_a_gpu_and_calls_the_loaded_library():
+    from omnihd_amd._lib import lib, torch_ops
+    face = torch_ops()
+    assert face is torch_ops() and {"token_embedding", "block_join", "topk_distill"} <= set(dir(face))
+    lib()
+    with pytest.raises(RuntimeError):                      # CPU tensors get no further than the device guard or the library's own checks
+        face.token_embedding(torch.zeros(3, dtype=torch.int64), torch.zeros(4, 8), 1.0, -1, torch.float32)
 
 
 def test_workspaces_cover_long_inputs():
