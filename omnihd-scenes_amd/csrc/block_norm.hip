@@ -30,13 +30,13 @@ struct BlockArgs {
   float *stats, *part;
   long long rows, xs, ys, gs, dxos, dhs; // row strides in elements (outputs are dense)
   long long per_gate, per_split;         // rows of one gate row, of one block
-  int splits, dim, post_type, gate_type, next_type, gate_kind;
+  int splits, dim, post_type, gate_type, next_type, gate_kind, stream;
   float r, eps;
 };
 
 template <int TPR> constexpr int threads_of() { return TPR > 256 ? TPR : 256; }
 
-template <typename TA, typename TX, int TPR, int NV, bool ODD, bool HASY>
+template <typename TA, typename TX, int TPR, int NV, bool ODD, bool HASY, bool STREAM>
 __global__ __launch_bounds__(threads_of<TPR>()) void k_block_fwd(BlockArgs a) {
   constexpr int TPB = threads_of<TPR>(), RPB = TPB / TPR;
   __shared__ float red[32];
@@ -69,8 +69,10 @@ __global__ __launch_bounds__(threads_of<TPR>()) void k_block_fwd(BlockArgs a) {
       xr[j] = typename Raw<TX>::V{};
       if (HASY) yr[j] = typename Raw<TA>::V{};
       if (row >= a.rows || left <= 0) continue;
-      xr[j] = raw8<ODD>(static_cast<const TX*>(a.x) + row * a.xs + c, left);
-      if (HASY) yr[j] = raw8<ODD>(static_cast<const TA*>(a.y) + row * a.ys + c, left);
+      const TX* x = static_cast<const TX*>(a.x) + row * a.xs + c;
+      const TA* y = static_cast<const TA*>(a.y) + (HASY ? row * a.ys + c : 0);
+      xr[j] = raw8<ODD, STREAM>(x, left);
+      if (HASY) yr[j] = raw8<ODD, STREAM>(y, left);
     }
   };
   const long long step = (long long)gridDim.x * RPB;
@@ -369,12 +371,13 @@ int lanes_of(int dim) {
   return l;
 }
 
-// Rows of one gate row are cut into as many blocks as fit the card at once (a backward lane needs up to 128 registers with a block's
-// output, about 64 without: 1024 or 2048 lanes a CU), but no block gets fewer rows than it has places for.
+// Rows of one gate row are cut into as many blocks as are on the card at once (with a block's output a backward lane needs 120 to 150
+// registers: three blocks of 256 a CU, one of 512 or 1024; four of 256 without), but no block gets fewer rows than it has places for.  More of
+// them cost their sums: 16384 x 4096 bf16, 256 / 512 / 768 blocks of 512: 195 / 202 / 236 us; 76800 x 256, 512 / 768 / 1024 of 256: 63 / 57 / 67.
 void split_of(long long rows, int dim, int gate_kind, long long per_gate, bool has_y, long long* groups, int* splits, long long* per_split) {
   const long long per = gate_kind == kGateRows ? per_gate : rows;
   *groups = rows > 0 ? (rows + per - 1) / per : 0;
-  const int tpr = lanes_of(dim), tpb = tpr > 256 ? tpr : 256, rpb = tpb / tpr, want = kCUs * (has_y ? 1024 : 2048) / tpb;
+  const int tpr = lanes_of(dim), tpb = tpr > 256 ? tpr : 256, rpb = tpb / tpr, want = kCUs * (tpb > 256 ? 1 : has_y ? 3 : 4);
   long long s = (want + *groups - 1) / (*groups > 0 ? *groups : 1), most = (per + rpb - 1) / rpb;
   if (s > most) s = most;
   if (s < 1) s = 1;
@@ -391,7 +394,9 @@ void launch(const BlockArgs& a, bool bwd, long long blocks, hipStream_t st) {
     hipLaunchKernelGGL((k_block_bwd<TA, TX, TPR, NV, ODD, HASY>), dim3((unsigned)blocks), dim3(TPB), wide, st, a);
   } else {
     long long g = (a.rows + RPB - 1) / RPB, most = (long long)kMaxBlocks * 256 / TPB;
-    hipLaunchKernelGGL((k_block_fwd<TA, TX, TPR, NV, ODD, HASY>), dim3((unsigned)(g < most ? g : most)), dim3(TPB), 0, st, a);
+    const dim3 grid((unsigned)(g < most ? g : most)), block(TPB);
+    if (!ODD && a.stream) hipLaunchKernelGGL((k_block_fwd<TA, TX, TPR, NV, ODD, HASY, !ODD>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((k_block_fwd<TA, TX, TPR, NV, ODD, HASY, false>), grid, block, 0, st, a);
   }
 }
 template <typename TA, typename TX, bool ODD, bool HASY>
@@ -457,6 +462,9 @@ extern "C" int omnihd_block_join_fwd(const void* x, long long x_stride, int x_ty
   a.rows = rows; a.xs = x_stride; a.ys = y_stride; a.gs = gate_stride; a.per_gate = rows_per_gate;
   a.dim = dim; a.post_type = post_type; a.gate_type = gate_type; a.next_type = next_type; a.gate_kind = gate_kind;
   a.r = residual_scale; a.eps = eps;
+  // inputs that the Infinity Cache cannot hold are read past it: 16384 x 4096 bf16 108 -> 92 us; below that they may well be there (8192 x 1024:
+  // 13.4 us, 16.3 past it)
+  a.stream = (size_t)rows * dim * (type_size(x_type) + (y ? type_size(act_type) : 0)) >= kCacheBytes;
   return run_block(a, x_type, act_type, false, 0, (hipStream_t)stream);
 }
 

@@ -19,7 +19,6 @@ namespace {
 using namespace tok;
 
 constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / 64;
-constexpr size_t kCacheBytes = 256u << 20;         // the Infinity Cache: a larger gradient's zero rows are stored past it
 constexpr int kMaxRange = 896;                     // table rows of one sorting block: 16 sets of counters, 56 KB of LDS
 
 template <typename ID> __device__ __forceinline__ bool usable(ID id, long long vocab, long long padding) {
@@ -83,29 +82,31 @@ __global__ __launch_bounds__(kSortThreads) void k_embed_sort(const ID* __restric
   const long long part = ((n + kSortWaves - 1) / kSortWaves + 63) / 64 * 64;
   const long long lo = part * w < n ? part * w : n, hi = lo + part < n ? lo + part : n;
   int* mine = hist + w * range;
-  int less = 0, found = 0;                         // (found: the same in all lanes)
-  for (long long b = lo; b < hi; b += 512) {       // eight loads in flight a lane
+  int less = 0, found = 0;                         // (the same in all lanes: counted from ballots)
+  // An id as 32 bits (all ones: none), so that one comparison each tells whether it is smaller than the range, or in it
+  const unsigned pad32 = padding < 0 ? ~0u : (unsigned)padding, vocab32 = (unsigned)vocab, first32 = (unsigned)r0, rows32 = (unsigned)rows;
+  auto narrow = [&](ID v) { const unsigned u = (unsigned)v; return v >= 0 && (sizeof(ID) == 4 || (unsigned long long)v >> 32 == 0) && u < vocab32 && u != pad32 ? u : ~0u; };
+  auto look = [&](ID v, long long at) {
+    const unsigned u = narrow(v), d = u - first32;
+    less += __popcll(__ballot(u < first32));
+    const unsigned long long who = __ballot(d < rows32);         // (no range ends at all ones: vocab < 2^31)
+    if (who == 0) return;
+    if (d < rows32) {
+      atomicAdd(mine + d, 1);
+      const int to = found + __popcll(who & before);
+      if (to < cap) { found_pos[to] = (int)at; found_row[to] = (short)d; }
+    }
+    found += __popcll(who);
+  };
+  long long b0 = lo;
+  for (; b0 + 512 <= hi; b0 += 512) {              // eight loads in flight a lane
     ID v[8];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] = b + 64 * k + lane < hi ? ids[b + 64 * k + lane] : (ID)-1;
+    for (int k = 0; k < 8; ++k) v[k] = ids[b0 + 64 * k + lane];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const bool ok = usable(v[k], vocab, padding);
-      const long long d = (long long)v[k] - r0;
-      less += ok && d < 0;
-      const bool in = ok && d >= 0 && d < rows;
-      const unsigned long long who = __ballot(in);
-      if (who == 0) continue;
-      if (in) {
-        atomicAdd(mine + d, 1);
-        const int at = found + __popcll(who & before);
-        if (at < cap) { found_pos[at] = (int)(b + 64 * k + lane); found_row[at] = (short)d; }
-      }
-      found += __popcll(who);
-    }
+    for (int k = 0; k < 8; ++k) look(v[k], b0 + 64 * k + lane);
   }
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) less += __shfl_xor(less, o, 64);
+  for (; b0 < hi; b0 += 64) look(b0 + lane < hi ? ids[b0 + lane] : (ID)-1, b0 + lane);
   if (lane == 0) smaller[w] = less;
   __syncthreads();
   // where each row's and wave's positions begin
@@ -164,8 +165,8 @@ __global__ __launch_bounds__(kSortThreads) void k_embed_sort(const ID* __restric
       for (int k = 0; k < 8; ++k) v[k] = b + 64 * k + lane < hi ? ids[b + 64 * k + lane] : (ID)-1;
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        const long long d = (long long)v[k] - r0;
-        const bool in = usable(v[k], vocab, padding) && d >= 0 && d < rows;
+        const unsigned d = narrow(v[k]) - first32;
+        const bool in = d < rows32;
         if (__ballot(in) != 0) place(in, in ? (int)d : 0, (int)(b + 64 * k + lane));
       }
     }

@@ -9,6 +9,7 @@ namespace omnihd {
 namespace tok {
 
 enum { kF32 = 0, kBF16 = 1, kF16 = 2 };          // omnihd_hip.h: element type codes
+constexpr size_t kCacheBytes = 256u << 20;       // the Infinity Cache
 inline bool type_ok(int t) { return t == kF32 || t == kBF16 || t == kF16; }
 inline int type_size(int t) { return t == kF32 ? 4 : 2; }
 
@@ -29,18 +30,18 @@ __device__ __forceinline__ void load8(const T* __restrict__ p, int left, float (
 
 // the same kept as they are (a row that is asked for ahead of its use), missing ones 0
 template <typename T> struct Raw { typedef T V __attribute__((ext_vector_type(8))); };
-template <bool ODD, typename T>
+template <bool ODD, bool STREAM = false, typename T>
 __device__ __forceinline__ typename Raw<T>::V raw8(const T* __restrict__ p, int left) {
   typedef typename Raw<T>::V V;
   typedef V W __attribute__((aligned(ODD ? sizeof(T) : 16)));
-  if (!ODD || left >= 8) return *reinterpret_cast<const W*>(p);
+  if (!ODD || left >= 8) return STREAM ? __builtin_nontemporal_load(reinterpret_cast<const W*>(p)) : *reinterpret_cast<const W*>(p);
   V v;
 #pragma unroll
   for (int k = 0; k < 8; ++k) v[k] = k < left ? p[k] : (T)0.f;
   return v;
 }
 
-// STREAM: past the caches, for an output that they would not hold anyway
+// STREAM: past the caches, for what they would not hold anyway
 template <bool ODD, bool STREAM = false, typename T>
 __device__ __forceinline__ void store8(T* __restrict__ p, int left, const float (&v)[8]) {
   if (!ODD || left >= 8) {

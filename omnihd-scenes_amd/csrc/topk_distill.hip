@@ -41,25 +41,26 @@ __device__ __forceinline__ float factor_of(const DistillArgs& a) { return a.avg 
 
 // 16 bytes of logits, kept as they are
 template <typename T> struct Pack { static constexpr int n = 16 / (int)sizeof(T); typedef T V __attribute__((ext_vector_type(16 / sizeof(T)))); };
+// `first` of them (if positive) and those from `left` on are not the row's: they read as -inf, and are not written
 template <bool ODD, typename T>
-__device__ __forceinline__ typename Pack<T>::V load_pack(const T* __restrict__ p, int left) {
+__device__ __forceinline__ typename Pack<T>::V load_pack(const T* __restrict__ p, int left, int first = 0) {
   typedef typename Pack<T>::V V;
   typedef V W __attribute__((aligned(ODD ? sizeof(T) : 16)));
-  if (!ODD || left >= Pack<T>::n) return *reinterpret_cast<const W*>(p);
+  if (!ODD || (left >= Pack<T>::n && first <= 0)) return *reinterpret_cast<const W*>(p);
   V v;
 #pragma unroll
-  for (int k = 0; k < Pack<T>::n; ++k) v[k] = k < left ? p[k] : (T)-__builtin_inff();
+  for (int k = 0; k < Pack<T>::n; ++k) v[k] = k < left && k >= first ? p[k] : (T)-__builtin_inff();
   return v;
 }
 // (past the caches: the gradient of a large vocabulary is read long after it is written - 1021 x 50021 fp16: 58 us, 49 with it)
 template <bool ODD, typename T>
-__device__ __forceinline__ void store_pack(T* __restrict__ p, int left, const typename Pack<T>::V& v) {
+__device__ __forceinline__ void store_pack(T* __restrict__ p, int left, const typename Pack<T>::V& v, int first = 0) {
   typedef typename Pack<T>::V V;
   typedef V W __attribute__((aligned(ODD ? sizeof(T) : 16)));
-  if (!ODD || left >= Pack<T>::n) { __builtin_nontemporal_store(v, reinterpret_cast<W*>(p)); return; }
+  if (!ODD || (left >= Pack<T>::n && first <= 0)) { __builtin_nontemporal_store(v, reinterpret_cast<W*>(p)); return; }
 #pragma unroll
   for (int k = 0; k < Pack<T>::n; ++k)
-    if (k < left) p[k] = v[k];
+    if (k < left && k >= first) p[k] = v[k];
 }
 
 // NaN where either is NaN (fmaxf drops it: a NaN logit has to reach the loss)
@@ -86,6 +87,9 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256, TPR > 256 ? 4 : 1) void k_di
     const long long row = first + sub;
     const bool act = row < a.rows;
     const T* z = static_cast<const T*>(a.z) + (act ? row : 0) * a.zs;
+    // Rows that start anywhere: packs are counted from the 16-byte border before the row (4096 x 50001 bf16: 225 us from its first entry)
+    const int skip = ODD ? (int)(reinterpret_cast<uintptr_t>(z) / sizeof(T) % VE) : 0, end = a.vocab + skip;
+    const T* zb = z - skip;
     const float w = !act ? 0.f : a.w ? a.w[row] : 1.f;
     // the row is asked for first: the teacher's slots are worked on while it is on its way
     V keep[KEEP];
@@ -93,8 +97,8 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256, TPR > 256 ? 4 : 1) void k_di
       if (w != 0.f) {
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-          const int at = (j * TPR + t) * VE, left = a.vocab - at;
-          if (left > 0) keep[j] = load_pack<ODD>(z + at, left);
+          const int at = (j * TPR + t) * VE, left = end - at;
+          if (left > 0) keep[j] = load_pack<ODD>(zb + at, left, skip - at);
         }
       }
     }
@@ -136,19 +140,19 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256, TPR > 256 ? 4 : 1) void k_di
       if constexpr (NV > 0) {
 #pragma unroll
         for (int j = 0; j < NV; ++j)
-          if ((j * TPR + t) * VE < a.vocab)
+          if ((j * TPR + t) * VE < end)
 #pragma unroll
             for (int k = 0; k < VE; ++k) m = fmaxf(m, (float)keep[j][k]);
       } else {
-        for (int at = t * VE; at < a.vocab; at += 4 * TPR * VE) {        // four loads in flight a lane
+        for (int at = t * VE; at < end; at += 4 * TPR * VE) {        // four loads in flight a lane
           V v[4];
           float big = -__builtin_inff();
 #pragma unroll
           for (int j = 0; j < 4; ++j)
-            if (at + j * TPR * VE < a.vocab) v[j] = load_pack<ODD>(z + at + j * TPR * VE, a.vocab - at - j * TPR * VE);
+            if (at + j * TPR * VE < end) v[j] = load_pack<ODD>(zb + at + j * TPR * VE, end - at - j * TPR * VE, skip - at - j * TPR * VE);
 #pragma unroll
           for (int j = 0; j < 4; ++j)
-            if (at + j * TPR * VE < a.vocab)
+            if (at + j * TPR * VE < end)
 #pragma unroll
               for (int k = 0; k < VE; ++k) big = fmaxf(big, (float)v[j][k]);
           if (big > m) {                           // (rescaled by the difference of the ROUNDED products that the terms are shifted by)
@@ -159,7 +163,7 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256, TPR > 256 ? 4 : 1) void k_di
           }
 #pragma unroll
           for (int j = 0; j < 4; ++j)
-            if (at + j * TPR * VE < a.vocab)
+            if (at + j * TPR * VE < end)
 #pragma unroll
               for (int k = 0; k < VE; ++k) s += __builtin_amdgcn_exp2f(fmaf((float)v[j][k], c, -own_mc));
         }
@@ -172,11 +176,11 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256, TPR > 256 ? 4 : 1) void k_di
       if constexpr (NV > 0) {
 #pragma unroll
         for (int j = 0; j < NV; ++j)
-          if ((j * TPR + t) * VE < a.vocab)
+          if ((j * TPR + t) * VE < end)
 #pragma unroll
             for (int k = 0; k < VE; ++k) s += __builtin_amdgcn_exp2f(fmaf((float)keep[j][k], c, -mc));
       } else if (own == -__builtin_inff()) {
-        if (m == own && t * VE < a.vocab) s = __builtin_nanf("");   // nothing but -inf in the row
+        if (m == own && t * VE < end) s = __builtin_nanf("");   // nothing but -inf in the row
       } else {
         s *= __builtin_amdgcn_exp2f(own_mc - mc);
       }
@@ -188,36 +192,36 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256, TPR > 256 ? 4 : 1) void k_di
     if (a.up) up = act ? a.up[a.up_step ? row : 0] : 0.f;
     const float k1 = coef == 0.f ? 0.f : scale * up, kq = k1 / s;
     if (a.g && act) {
-      T* g = static_cast<T*>(a.g) + row * a.gs;
+      T* g = static_cast<T*>(a.g) + row * a.gs - skip;
       if (k1 == 0.f) {                             // nothing to learn from this row
         V zero;
 #pragma unroll
         for (int k = 0; k < VE; ++k) zero[k] = (T)0.f;
-        for (int at = t * VE; at < a.vocab; at += TPR * VE) store_pack<ODD>(g + at, a.vocab - at, zero);
+        for (int at = t * VE; at < end; at += TPR * VE) store_pack<ODD>(g + at, end - at, zero, skip - at);
       } else if constexpr (NV > 0) {
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-          const int at = (j * TPR + t) * VE, left = a.vocab - at;
+          const int at = (j * TPR + t) * VE, left = end - at;
           if (left <= 0) continue;
           V o;
 #pragma unroll
           for (int k = 0; k < VE; ++k) o[k] = (T)(__builtin_amdgcn_exp2f(fmaf((float)keep[j][k], c, -mc)) * kq);
-          store_pack<ODD>(g + at, left, o);
+          store_pack<ODD>(g + at, left, o, skip - at);
         }
       } else {
-        for (int at = t * VE; at < a.vocab; at += 4 * TPR * VE) {
+        for (int at = t * VE; at < end; at += 4 * TPR * VE) {
           V v[4];
 #pragma unroll
           for (int j = 0; j < 4; ++j)
-            if (at + j * TPR * VE < a.vocab) v[j] = load_pack<ODD>(z + at + j * TPR * VE, a.vocab - at - j * TPR * VE);
+            if (at + j * TPR * VE < end) v[j] = load_pack<ODD>(zb + at + j * TPR * VE, end - at - j * TPR * VE, skip - at - j * TPR * VE);
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const int left = a.vocab - at - j * TPR * VE;
+            const int left = end - at - j * TPR * VE;
             if (left <= 0) continue;
             V o;
 #pragma unroll
             for (int k = 0; k < VE; ++k) o[k] = (T)(__builtin_amdgcn_exp2f(fmaf((float)v[j][k], c, -mc)) * kq);
-            store_pack<ODD>(g + at + j * TPR * VE, left, o);
+            store_pack<ODD>(g + at + j * TPR * VE, left, o, skip - at - j * TPR * VE);
           }
         }
       }
@@ -232,6 +236,14 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256, TPR > 256 ? 4 : 1) void k_di
       float part = 0.f;
       if (coef != 0.f && act) {
         const float lq = __builtin_amdgcn_logf(s);
+        unsigned long long alone = 0;              // the lanes whose id stands in the row once: one comparison a slot tells them
+        if (SL == 64 && K <= 64) {
+          const int mine = t < K ? sid[t] : -1;
+          for (int o = 0; o < K; ++o) {
+            const unsigned long long same = __ballot(mine == __builtin_amdgcn_readlane(mine, o));
+            if ((same & (same - 1)) == 0) alone |= same;
+          }
+        }
         for (int k = t; k < K; k += SL) {
           const int id = sid[k];
           if (id < 0) continue;
@@ -240,6 +252,8 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256, TPR > 256 ? 4 : 1) void k_di
           if (!a.g || k1 == 0.f) continue;
           float sum = 0.f;                         // p of every slot with this id; only the first of them writes
           bool leads = true;
+          if (alone >> t & 1) sum = p;
+          else
           for (int o = 0; o < K; ++o)
             if (sid[o] == id) {
               leads &= o >= k;
@@ -292,6 +306,14 @@ __global__ __launch_bounds__(256) void k_distill_lanes(DistillArgs a) {
     const float w = !act ? 0.f : a.w ? a.w[row] : 1.f;
     const T* z = static_cast<const T*>(a.z) + row * a.zs;
     const int held = (int)(a.rows - first < 64 ? a.rows - first : 64) * a.vocab;      // elements of this wave's rows
+    const int K = a.top, V_ = a.vocab;
+    long long raw_id[KR];                          // the teacher's slots are asked for before the rows
+    float raw_t[KR];
+#pragma unroll
+    for (int k = 0; k < KR; ++k) {
+      raw_id[k] = k < K ? id_at(a, row * a.is + k) : -1;
+      raw_t[k] = k < K ? load1_any(a.t, a.t_type, row * a.ts + k) : 0.f;
+    }
     if (in_dense) {
       for (int e = lane * VE; e < held; e += 64 * VE) {
         const V v = load_pack<true>(static_cast<const T*>(a.z) + first * a.vocab + e, held - e);
@@ -304,37 +326,33 @@ __global__ __launch_bounds__(256) void k_distill_lanes(DistillArgs a) {
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       __builtin_amdgcn_wave_barrier();
     }
-    const int K = a.top, V_ = a.vocab;
     float x[VM], m = -__builtin_inff(), s = 0.f;
     int id[KR];
     float tv[KR], mt = -__builtin_inff();
     bool bad = false;
-    if (in_dense) {
+    if (!in_dense) {
 #pragma unroll
-      for (int k = 0; k < VM; ++k) x[k] = k < V_ ? tile[(int)(row - first) * PITCH + k] : -__builtin_inff();
-    } else
+      for (int j = 0; j < NP; ++j)
+        if (j * VE < V_) {
+          const V v = load_pack<true>(z + j * VE, V_ - j * VE);
 #pragma unroll
-    for (int j = 0; j < NP; ++j) {
-      if (j * VE < V_) {
-        const V v = load_pack<true>(z + j * VE, V_ - j * VE);
-#pragma unroll
-        for (int k = 0; k < VE; ++k) x[j * VE + k] = (float)v[k];
-      } else {
-#pragma unroll
-        for (int k = 0; k < VE; ++k) x[j * VE + k] = -__builtin_inff();
-      }
+          for (int k = 0; k < VE; ++k) tile[lane * PITCH + j * VE + k] = (float)v[k];
+        }
     }
-    auto slot = [&](int k, int& i, float& v) {
-      const long long full = id_at(a, row * a.is + k);
-      v = full < 0 ? -__builtin_inff() : load1_any(a.t, a.t_type, row * a.ts + k);
+    if (!act && in_dense)                          // (the last row's copy: its entries in this lane's own place)
+      for (int k = 0; k < V_; ++k) tile[lane * PITCH + k] = 0.f;
+#pragma unroll
+    for (int k = 0; k < VM; ++k) x[k] = k < V_ ? tile[lane * PITCH + k] : -__builtin_inff();
+    auto take = [&](long long full, float value, int& i, float& v) {
+      v = full < 0 ? -__builtin_inff() : value;
       bad |= full >= V_;
       i = full < 0 || full >= V_ ? -1 : (int)full;
     };
+    auto slot = [&](int k, int& i, float& v) { take(id_at(a, row * a.is + k), load1_any(a.t, a.t_type, row * a.ts + k), i, v); };
 #pragma unroll
-    for (int k = 0; k < KR; ++k) {
-      id[k] = -1; tv[k] = -__builtin_inff();
-      if (k < K) { slot(k, id[k], tv[k]); mt = MaxNan()(mt, tv[k]); }
-    }
+    for (int k = 0; k < KR; ++k) take(raw_id[k], raw_t[k], id[k], tv[k]);
+#pragma unroll
+    for (int k = 0; k < KR; ++k) mt = MaxNan()(mt, tv[k]);
     for (int k = KR; k < K; ++k) {
       int i; float v;
       slot(k, i, v);
@@ -363,19 +381,15 @@ __global__ __launch_bounds__(256) void k_distill_lanes(DistillArgs a) {
     float up = 1.f;
     if (a.up) up = a.up[a.up_step ? row : 0];
     const float k1 = coef == 0.f ? 0.f : base * coef * a.temperature * up, kq = k1 / s;
-    float mass[VM], part = 0.f;
-#pragma unroll
-    for (int k = 0; k < VM; ++k) mass[k] = 0.f;
+    float part = 0.f;
+    float* own = tile + lane * PITCH;              // this lane's row: logits here, its gradient below
     auto use = [&](int i, float v) {
       if (i < 0) return;
-      const float lp = fmaf(v, c, -mtc) - ls, p = __builtin_amdgcn_exp2f(lp);
-      float zk = 0.f;
-#pragma unroll
-      for (int q = 0; q < VM; ++q) {
-        mass[q] += q == i ? p : 0.f;
-        zk = q == i ? x[q] : zk;
-      }
+      const float lp = fmaf(v, c, -mtc) - ls, p = __builtin_amdgcn_exp2f(lp), zk = fmaf(own[i], c, -mc);
       if (!(p == 0.f)) part = fmaf(p, lp - (zk - lq), part);
+    };
+    auto learn = [&](int i, float v) {
+      if (i >= 0) own[i] -= k1 * __builtin_amdgcn_exp2f(fmaf(v, c, -mtc) - ls);
     };
     if (coef != 0.f) {
 #pragma unroll
@@ -389,12 +403,19 @@ __global__ __launch_bounds__(256) void k_distill_lanes(DistillArgs a) {
     if (a.g) {
       T* g = static_cast<T*>(a.g) + row * a.gs;
 #pragma unroll
-      for (int k = 0; k < VM; ++k) {
-        const float v = k1 == 0.f ? 0.f : fmaf(__builtin_amdgcn_exp2f(x[k]), kq, -k1 * mass[k]);
-        if (k < V_ && act) {
-          if (out_dense) tile[lane * PITCH + k] = v;
-          else g[k] = (T)v;
+      for (int k = 0; k < VM; ++k)
+        if (k < V_) own[k] = k1 == 0.f ? 0.f : __builtin_amdgcn_exp2f(x[k]) * kq;
+      if (k1 != 0.f) {
+#pragma unroll
+        for (int k = 0; k < KR; ++k) if (k < K) learn(id[k], tv[k]);
+        for (int k = KR; k < K; ++k) {
+          int i; float v;
+          slot(k, i, v);
+          learn(i, v);
         }
+      }
+      if (!out_dense && act) {
+        for (int k = 0; k < V_; ++k) g[k] = (T)own[k];
       }
       if (out_dense) {
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -439,12 +460,14 @@ __global__ __launch_bounds__(1024) void k_distill_total(const float* __restrict_
 }
 
 struct Geometry { int tpr, nv; };       // nv 0: the row is read twice
-template <typename T> Geometry geometry(int vocab, int top) {
-  const long long packs = (vocab + Pack<T>::n - 1) / Pack<T>::n;
+// A lane holds up to eight packs, sixteen in the longest rows.  Short rows share a wave, so that the teacher's part, much the same for any
+// vocabulary, is paid once for several (60000 x 1000 bf16: 96 us with a wave a row).
+template <typename T> Geometry geometry(int vocab, int top, bool odd) {
+  const long long packs = odd ? (vocab + 2ll * (Pack<T>::n - 1)) / Pack<T>::n : vocab / Pack<T>::n;       // (odd: at any start of the row)
   int tpr = 8;
-  while (tpr < 64 && (packs > tpr || (256 / tpr) * 12 * top > 32768)) tpr *= 2;
-  if (packs <= tpr) return {tpr, 1};
-  if (packs <= 64 * 4) return {64, 4};
+  while (tpr < 64 && (packs > 8 * tpr || (256 / tpr) * 12 * top > 32768)) tpr *= 2;
+  if (tpr == 8 && packs <= 8 * 2) return {8, 2};
+  if (packs <= 8 * tpr) return {tpr, 8};
   if (packs <= 256 * 4) return {256, 4};
   if (packs <= 256 * 8) return {256, 8};
   if (packs <= 512 * 8) return {512, 8};
@@ -453,28 +476,32 @@ template <typename T> Geometry geometry(int vocab, int top) {
   return {1024, 0};
 }
 bool by_lanes(int vocab) { return vocab <= 32; }
-template <typename T> int blocks_of(long long rows, int vocab, int top) {
+template <typename T> int blocks_of(long long rows, int vocab, int top, bool odd) {
   if (by_lanes(vocab)) return (int)(rows <= 16384 * 256 ? (rows + 255) / 256 : 16384);
-  const int tpr = geometry<T>(vocab, top).tpr, tpb = tpr > 256 ? tpr : 256;
+  const int tpr = geometry<T>(vocab, top, odd).tpr, tpb = tpr > 256 ? tpr : 256;
   const long long g = (rows + tpb / tpr - 1) / (tpb / tpr), most = (long long)kMaxBlocks * 256 / tpb;
   return (int)(g < most ? g : most);
 }
-int blocks_of_type(int type, long long rows, int vocab, int top) {
+template <typename T> int most_blocks(long long rows, int vocab, int top) {
   if (rows <= 0) return 1;
-  return type == kF32 ? blocks_of<float>(rows, vocab, top) : blocks_of<__bf16>(rows, vocab, top);
+  const int odd = blocks_of<T>(rows, vocab, top, true);
+  if (vocab % Pack<T>::n) return odd;
+  const int even = blocks_of<T>(rows, vocab, top, false);
+  return odd > even ? odd : even;
 }
 
 template <typename T, bool ODD>
-void launch_rows(const DistillArgs& a, int blocks, hipStream_t st) {
-  const Geometry g = geometry<T>(a.vocab, a.top);
+int launch_rows(const DistillArgs& a, hipStream_t st) {
+  const Geometry g = geometry<T>(a.vocab, a.top, ODD);
+  const int blocks = blocks_of<T>(a.rows, a.vocab, a.top, ODD);
   const int tpb = g.tpr > 256 ? g.tpr : 256;
   const size_t lds = (size_t)(tpb / g.tpr) * 3 * a.top * sizeof(float);
 #define OMNIHD_DISTILL(R, N) hipLaunchKernelGGL((k_distill_rows<T, R, N, ODD>), dim3(blocks), dim3(tpb), lds, st, a)
-  if (g.tpr == 8) OMNIHD_DISTILL(8, 1);
-  else if (g.tpr == 16) OMNIHD_DISTILL(16, 1);
-  else if (g.tpr == 32) OMNIHD_DISTILL(32, 1);
-  else if (g.tpr == 64 && g.nv == 1) OMNIHD_DISTILL(64, 1);
-  else if (g.tpr == 64) OMNIHD_DISTILL(64, 4);
+  if (g.tpr == 8 && g.nv == 2) OMNIHD_DISTILL(8, 2);
+  else if (g.tpr == 8) OMNIHD_DISTILL(8, 8);
+  else if (g.tpr == 16) OMNIHD_DISTILL(16, 8);
+  else if (g.tpr == 32) OMNIHD_DISTILL(32, 8);
+  else if (g.tpr == 64) OMNIHD_DISTILL(64, 8);
   else if (g.tpr == 256 && g.nv == 4) OMNIHD_DISTILL(256, 4);
   else if (g.tpr == 256) OMNIHD_DISTILL(256, 8);
   else if (g.nv == 8) OMNIHD_DISTILL(512, 8);
@@ -482,17 +509,20 @@ void launch_rows(const DistillArgs& a, int blocks, hipStream_t st) {
   else if (g.nv == 16) OMNIHD_DISTILL(1024, 16);
   else OMNIHD_DISTILL(1024, 0);
 #undef OMNIHD_DISTILL
+  return blocks;
 }
+// the number of blocks, each of which leaves a sum
 template <typename T>
-void launch_distill(const DistillArgs& a, int blocks, hipStream_t st) {
+int launch_distill(const DistillArgs& a, hipStream_t st) {
   if (by_lanes(a.vocab)) {
+    const int blocks = blocks_of<T>(a.rows, a.vocab, a.top, true);
     if (a.vocab <= 16) hipLaunchKernelGGL((k_distill_lanes<T, 16>), dim3(blocks), dim3(256), 0, st, a);
     else hipLaunchKernelGGL((k_distill_lanes<T, 32>), dim3(blocks), dim3(256), 0, st, a);
-    return;
+    return blocks;
   }
   auto fits = [&](const void* p, long long stride) { return !p || ((reinterpret_cast<uintptr_t>(p) & 15u) == 0 && stride % Pack<T>::n == 0); };
-  if (a.vocab % Pack<T>::n == 0 && fits(a.z, a.zs) && fits(a.g, a.gs)) launch_rows<T, false>(a, blocks, st);
-  else launch_rows<T, true>(a, blocks, st);
+  if (a.vocab % Pack<T>::n == 0 && fits(a.z, a.zs) && fits(a.g, a.gs)) return launch_rows<T, false>(a, st);
+  return launch_rows<T, true>(a, st);
 }
 
 }  // namespace
@@ -502,7 +532,8 @@ using namespace omnihd;
 
 extern "C" size_t omnihd_topk_distill_workspace_bytes(long long rows, int vocab, int top, int z_type) {
   if (rows < 0 || vocab < 1 || top < 1 || top > kMaxTop || !type_ok(z_type)) return 0;
-  return align_up((size_t)blocks_of_type(z_type, rows, vocab, top) * sizeof(float), 256);
+  const int blocks = z_type == kF32 ? most_blocks<float>(rows, vocab, top) : most_blocks<__bf16>(rows, vocab, top);
+  return align_up((size_t)blocks * sizeof(float), 256);
 }
 
 extern "C" int omnihd_topk_distill(const void* z, int z_type, long long z_stride, const void* t, int t_type, long long t_stride,
@@ -515,7 +546,7 @@ extern "C" int omnihd_topk_distill(const void* z, int z_type, long long z_stride
   OMNIHD_REQUIRE(temperature > 0.f, "temperature > 0");
   OMNIHD_REQUIRE(!skip_if_one || (up && !up_per_row && !loss && !row_loss), "skip_if_one goes with one gradient for all rows");
   hipStream_t st = (hipStream_t)stream;
-  const int blocks = blocks_of_type(z_type, rows, vocab, top);
+  int blocks = 0;
   float* sums = nullptr;
   if (loss) {
     const size_t need = omnihd_topk_distill_workspace_bytes(rows, vocab, top, z_type);
@@ -530,10 +561,8 @@ extern "C" int omnihd_topk_distill(const void* z, int z_type, long long z_stride
     a.rows = rows; a.zs = z_stride; a.gs = grad_stride; a.ts = t_stride; a.is = ids_stride;
     a.vocab = vocab; a.top = top; a.t_type = t_type; a.wide_ids = wide_ids; a.up_step = up_per_row; a.skip_if_one = skip_if_one;
     a.temperature = temperature; a.factor = factor;
-    if (z_type == kF32) launch_distill<float>(a, blocks, st);
-    else if (z_type == kBF16) launch_distill<__bf16>(a, blocks, st);
-    else launch_distill<_Float16>(a, blocks, st);
+    blocks = z_type == kF32 ? launch_distill<float>(a, st) : z_type == kBF16 ? launch_distill<__bf16>(a, st) : launch_distill<_Float16>(a, st);
   }
-  if (loss) hipLaunchKernelGGL(k_distill_total, dim3(1), dim3(1024), 0, st, sums, rows > 0 ? blocks : 0, loss);
+  if (loss) hipLaunchKernelGGL(k_distill_total, dim3(1), dim3(1024), 0, st, sums, blocks, loss);
   return check_launch("topk_distill");
 }

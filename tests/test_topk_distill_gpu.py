@@ -191,14 +191,16 @@ def test_shapes_strides_and_no_rows(cuda):
         wide = torch.zeros(40 * pitch + offset, dtype=B, device="cuda")[offset:].view(40, pitch)
         wide[:, :vocab] = z
         wide[:, vocab:] = 99
-        ref_z = z.requires_grad_()
-        ref = ops.topk_distill_loss(ref_z, t, ids)
-        ref_g, = torch.autograd.grad(ref, ref_z)
         view = wide[:, :vocab].detach().requires_grad_()
         tw, iw = torch.zeros(40, 9, device="cuda")[:, 1:7], torch.zeros(40, 8, dtype=ids.dtype, device="cuda")[:, 2:8]
         tw.copy_(t), iw.copy_(ids)
         got = ops.topk_distill_loss(view, tw, iw)
-        assert torch.equal(got, ref) and torch.equal(torch.autograd.grad(got, view)[0], ref_g)
+        grad, = torch.autograd.grad(got, view)
+        # which lane adds which entry goes by the row's address: the same bounds as for dense rows, not the same bits
+        rows, row_terms, dz, dz_terms = reference(z, t, ids, 1.0, None, 1 / 40)
+        check_close(got, rows.sum(), bound(rows.sum(), F, row_terms.sum(), ROUNDINGS + 40), "loss")
+        check_close(grad, dz, bound(dz, B, dz_terms, ROUNDINGS), "gradient")
+        assert grad.shape == (40, vocab) and bool((wide[:, vocab:] == 99).all())
     z = torch.zeros(0, 50, device="cuda").requires_grad_()
     empty = (torch.zeros(0, 4, device="cuda"), torch.zeros(0, 4, dtype=torch.int64, device="cuda"))
     loss = ops.topk_distill_loss(z, *empty)
