@@ -19,6 +19,7 @@ namespace {
 using namespace tok;
 
 constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / 64;
+constexpr int kMaxWidth = 1 << 24;                 // (columns are counted in int)
 constexpr int kMaxRange = 896;                     // table rows of one sorting block: 16 sets of counters, 56 KB of LDS
 
 template <typename ID> __device__ __forceinline__ bool usable(ID id, long long vocab, long long padding) {
@@ -139,10 +140,20 @@ __global__ __launch_bounds__(kSortThreads) void k_embed_sort(const ID* __restric
   while ((1 << bits) < rows) ++bits;
   // 64 tokens of this wave in order: each to the place that its row has reached
   auto place = [&](bool in, int d, int at) {
-    unsigned long long same = __ballot(in);
-    for (int k = 0; k < bits; ++k) {               // the lanes with this lane's row
-      const unsigned long long set = __ballot(in && ((d >> k) & 1));
-      same &= ((d >> k) & 1) ? set : ~set;
+    unsigned long long same = 0, todo = __ballot(in);
+    for (int k = 0; k < 3 && todo; ++k) {          // a frequent token or two, one comparison each ...
+      const unsigned long long like = __ballot(in && d == __builtin_amdgcn_readlane(d, __builtin_ctzll(todo)));
+      if (like >> lane & 1) same = like;
+      todo &= ~like;
+    }
+    if (todo) {                                    // ... and the rest by the bits of their rows: the lanes with this lane's row
+      const bool rest = todo >> lane & 1;
+      unsigned long long mine_too = todo;
+      for (int k = 0; k < bits; ++k) {
+        const unsigned long long set = __ballot(rest && ((d >> k) & 1));
+        mine_too &= ((d >> k) & 1) ? set : ~set;
+      }
+      if (rest) same = mine_too;
     }
     if (in) {
       const int nth = __popcll(same & before), from = mine[d];
@@ -150,24 +161,30 @@ __global__ __launch_bounds__(kSortThreads) void k_embed_sort(const ID* __restric
       if (nth == 0) mine[d] = from + __popcll(same);
       __builtin_amdgcn_wave_barrier();
       keys[from + nth] = (int)(r0 + d);
-      pos[from + nth] = LISTED ? where[at] : at;
+      pos[from + nth] = at;
     }
   };
   if (found <= cap) {
     for (int b = 0; b < found; b += 64) {
       const bool in = b + lane < found;
-      place(in, in ? found_row[b + lane] : 0, in ? found_pos[b + lane] : 0);
+      const int at = in ? found_pos[b + lane] : 0;
+      place(in, in ? found_row[b + lane] : 0, LISTED && in ? where[at] : at);
     }
   } else {                                         // a crowded range: the ids once more
     for (long long b = lo; b < hi; b += 512) {
       ID v[8];
+      int at[8];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] = b + 64 * k + lane < hi ? ids[b + 64 * k + lane] : (ID)-1;
+      for (int k = 0; k < 8; ++k) {
+        const long long i = b + 64 * k + lane;
+        v[k] = i < hi ? ids[i] : (ID)-1;
+        at[k] = LISTED && i < hi ? where[i] : (int)i;
+      }
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
         const unsigned d = narrow(v[k]) - first32;
         const bool in = d < rows32;
-        if (__ballot(in) != 0) place(in, in ? (int)d : 0, (int)(b + 64 * k + lane));
+        if (__ballot(in) != 0) place(in, in ? (int)d : 0, at[k]);
       }
     }
   }
@@ -408,18 +425,16 @@ int range_for(long long vocab) {
   long long r = (vocab + 2 * kCUs - 1) / (2 * kCUs);
   return (int)(r > kMaxRange ? kMaxRange : r < 1 ? 1 : r);
 }
-// tokens that a wave of a sorting block can keep: what is left of 64 KB, no more than 256
-int cap_for(int range) {
-  const int c = (64000 - (kSortWaves + 1) * range * 4) / (kSortWaves * 6);
-  return (c > 256 ? 256 : c) & ~1;
-}
-// sorted positions of one chunk: short ones while few, so that they fill the card; at most some thousands of parts to join
-int chunk_for(long long n) {
-  int c = 16;
-  while (c < 256 && n / c > 1024) c *= 2;
+// tokens that a wave of a sorting block can keep: what is left of 64 KB (two blocks a CU)
+int cap_for(int range) { return (64000 - (kSortWaves + 1) * range * 4) / (kSortWaves * 6) & ~1; }
+// sorted positions of one chunk: as many chunks x slabs as give 4096 waves where the row is wide, no fewer than 8 positions, no more than 256
+// (72946 positions of 52 columns: 135 us in chunks of 128, whose 570 groups of 8 lanes fill 18 blocks)
+int chunk_for(long long n, int dim) {
+  const int l = lanes_for(dim, 64), slabs = (dim + l * 8 - 1) / (l * 8);
+  int c = 8;
+  while (c < 256 && (n / (2 * c)) * slabs * l >= 4096ll * 64) c *= 2;
   return c;
 }
-
 // From here on the ids are put into buckets first: three more launches, but no block reads all of them.
 constexpr long long kBucketIds = 1 << 17;
 int span_for(long long vocab) {
@@ -432,7 +447,8 @@ BwdWs bwd_ws(long long n, long long vocab, int dim) {
   BwdWs w{};
   size_t at = 0;
   auto take = [&](size_t bytes) { const size_t from = at; at += align_up(bytes, 256); return from; };
-  w.chunks = (n + chunk_for(n) - 1) / chunk_for(n);
+  const int chunk = chunk_for(n, dim);
+  w.chunks = (n + chunk - 1) / chunk;
   w.keys = take((size_t)n * 4);
   w.pos = take((size_t)n * 4);
   w.used = take(4);
@@ -475,7 +491,7 @@ int bwd(const void* ids, const void* g, long long pitch, long long vocab, long l
         char* ws, const BwdWs& at, hipStream_t st) {
   int *keys = reinterpret_cast<int*>(ws + at.keys), *pos = reinterpret_cast<int*>(ws + at.pos), *used = reinterpret_cast<int*>(ws + at.used);
   float* parts = reinterpret_cast<float*>(ws + at.parts);
-  const int range = range_for(vocab), cap = cap_for(range), chunk = chunk_for(n);
+  const int range = range_for(vocab), cap = cap_for(range), chunk = chunk_for(n, dim);
   const dim3 sorters((unsigned)((vocab + range - 1) / range));
   const size_t lds = (size_t)(kSortWaves + 1) * range * sizeof(int) + (size_t)kSortWaves * cap * 6;
   const int stream = (size_t)vocab * dim * sizeof(TT) > kCacheBytes;
@@ -532,7 +548,8 @@ bool row_vec(const void* p, long long pitch, int dim, int type) {
 using namespace omnihd;
 
 #define OMNIHD_EMBED_CHECKS                                                                                                          \
-  OMNIHD_REQUIRE(n >= 0 && n < (1ll << 31) && vocab >= 1 && vocab < (1ll << 31) && dim >= 1, "0 <= n < 2^31, 1 <= vocab < 2^31, dim >= 1"); \
+  OMNIHD_REQUIRE(n >= 0 && n < (1ll << 31) && vocab >= 1 && vocab < (1ll << 31) && dim >= 1 && dim <= kMaxWidth,                         \
+                 "0 <= n < 2^31, 1 <= vocab < 2^31, 1 <= dim <= 2^24");                                                                      \
   OMNIHD_REQUIRE(type_ok(table_type) && type_ok(out_type) && (table_type == out_type || table_type == kF32), "types: the table has the output's type or fp32")
 
 extern "C" int omnihd_token_embed_fwd(const void* ids, int wide_ids, long long n, const void* table, int table_type, long long table_stride,
@@ -549,7 +566,7 @@ extern "C" int omnihd_token_embed_fwd(const void* ids, int wide_ids, long long n
 }
 
 extern "C" size_t omnihd_token_embed_bwd_workspace_bytes(long long n, long long vocab, int dim) {
-  return n < 0 || n >= (1ll << 31) || vocab < 1 || vocab >= (1ll << 31) || dim < 1 ? 0 : bwd_ws(n, vocab, dim).total;
+  return n < 0 || n >= (1ll << 31) || vocab < 1 || vocab >= (1ll << 31) || dim < 1 || dim > kMaxWidth ? 0 : bwd_ws(n, vocab, dim).total;
 }
 
 extern "C" int omnihd_token_embed_bwd(const void* ids, int wide_ids, long long n, const void* g, int out_type, long long g_stride,

@@ -21,7 +21,7 @@ namespace omnihd {
 namespace {
 using namespace tok;
 
-constexpr int kMaxTop = 256;
+constexpr int kMaxTop = 256, kMaxVocab = 1 << 30;      // (places in a row are counted in int)
 constexpr float kLn2 = 0.69314718055994531f;
 
 struct DistillArgs {
@@ -531,7 +531,7 @@ int launch_distill(const DistillArgs& a, hipStream_t st) {
 using namespace omnihd;
 
 extern "C" size_t omnihd_topk_distill_workspace_bytes(long long rows, int vocab, int top, int z_type) {
-  if (rows < 0 || vocab < 1 || top < 1 || top > kMaxTop || !type_ok(z_type)) return 0;
+  if (rows < 0 || vocab < 1 || vocab > kMaxVocab || top < 1 || top > kMaxTop || !type_ok(z_type)) return 0;
   const int blocks = z_type == kF32 ? most_blocks<float>(rows, vocab, top) : most_blocks<__bf16>(rows, vocab, top);
   return align_up((size_t)blocks * sizeof(float), 256);
 }
@@ -541,7 +541,8 @@ extern "C" int omnihd_topk_distill(const void* z, int z_type, long long z_stride
                                    int top, float temperature, float factor, const float* avg_factor, const float* up, int up_per_row,
                                    int skip_if_one, void* grad, long long grad_stride, float* row_loss, float* loss, void* workspace,
                                    size_t workspace_bytes, void* stream) {
-  OMNIHD_REQUIRE(rows >= 0 && rows < (1ll << 31) && vocab >= 1 && top >= 1 && top <= kMaxTop, "0 <= rows < 2^31, vocab >= 1, 1 <= top <= 256");
+  OMNIHD_REQUIRE(rows >= 0 && rows < (1ll << 31) && vocab >= 1 && vocab <= kMaxVocab && top >= 1 && top <= kMaxTop,
+                 "0 <= rows < 2^31, 1 <= vocab <= 2^30, 1 <= top <= 256");
   OMNIHD_REQUIRE(type_ok(z_type) && type_ok(t_type), "types");
   OMNIHD_REQUIRE(temperature > 0.f, "temperature > 0");
   OMNIHD_REQUIRE(!skip_if_one || (up && !up_per_row && !loss && !row_loss), "skip_if_one goes with one gradient for all rows");

@@ -264,19 +264,25 @@ struct Distill : public Function<Distill> {
     Tensor loss, grad;
     if (fresh) grad = dense_like(z);
     distill_run(z, t, ids, weight, avg, temperature, factor, per_row, &loss, grad, Tensor(), false);
-    ctx->save_for_backward({z, t, ids, weight, avg, grad});
+    ctx->save_for_backward({z, t, ids, weight, avg});
     ctx->saved_data["temperature"] = temperature;
     ctx->saved_data["factor"] = factor;
     ctx->saved_data["per_row"] = per_row;
-    ctx->saved_data["fresh"] = fresh;
+    if (fresh) ctx->saved_data["grad"] = grad;      // (not among the saved variables: its next holder may write to it)
     return loss;
   }
   static variable_list backward(AutogradContext* ctx, variable_list ups) {
     no_second_order("topk_distill_loss");
     const variable_list in = ctx->get_saved_variables();
-    const bool in_place = ctx->saved_data["fresh"].toBool() && !capturing();
-    if (in_place) ctx->saved_data["fresh"] = false;
-    Tensor grad = in_place ? in[5] : dense_like(in[0]);
+    Tensor grad;
+    const auto kept = ctx->saved_data.find("grad");
+    const bool in_place = kept != ctx->saved_data.end() && !capturing();
+    if (in_place) {
+      grad = kept->second.toTensor();
+      ctx->saved_data.erase(kept);
+    } else {
+      grad = dense_like(in[0]);
+    }
     distill_run(in[0], in[1], in[2], in[3], in[4], ctx->saved_data["temperature"].toDouble(), ctx->saved_data["factor"].toDouble(),
                 ctx->saved_data["per_row"].toBool(), nullptr, grad, ups[0].contiguous(), in_place);
     variable_list grads(8);

@@ -13,6 +13,7 @@ from torch import nn
 
 from omnihd_amd.mm import ConvModule
 from omnihd_amd.mm.registry import HEADS, LOSSES, build_from_cfg
+from omnihd_amd.ops import topk_distill_loss
 
 
 def _nll_of_one(x):
@@ -54,6 +55,17 @@ class BEVOCCHead2Dv2(nn.Module):
         loss_ssc = self.sem_scal_loss(occ_pred, sem) + self.geo_scal_loss(occ_pred, sem)
         loss_occ = self.loss_occ(occ_pred.reshape(-1, self.num_classes), sem.reshape(-1))
         return dict(loss_ssc=loss_ssc, loss_occ=loss_occ)
+
+    def distill_loss(self, occ_pred, teacher_logits, teacher_classes, known=None, temperature=1.0, loss_weight=1.0):
+        """Distillation from a teacher (a detector with a sensor more, say) of which each voxel's top K class logits were kept:
+        teacher_logits, teacher_classes (B, Dx, Dy, Dz, K); ``known`` (B, Dx, Dy, Dz): the voxels that count (default all; the loss
+        is their mean).  See ops.topk_distill_loss; the reference has no counterpart."""
+        avg = None
+        if known is not None:
+            known = known.float()
+            avg = known.sum().clamp_min(1.0)
+        return dict(loss_occ_distill=topk_distill_loss(occ_pred, teacher_logits, teacher_classes, temperature=temperature, row_weight=known,
+                                                       avg_factor=avg, loss_weight=loss_weight))
 
     @staticmethod
     def geo_scal_loss(preds, ssc_target, semantic=True):

@@ -98,7 +98,7 @@ def test_c_entries_refuse_before_any_launch():
     p = ctypes.c_void_p(64)                                # never read: every call below is refused first
     ARG, WORKSPACE = -1, -3
     embed = [p, 1, 5, p, 0, 8, 4, 8, 1.0, p, 0, None]
-    for at, bad in ((2, -1), (2, 1 << 31), (6, 0), (6, 1 << 31), (7, 0), (4, 3), (10, 2 + 5), (4, 1), (5, 7), (0, None), (3, None), (9, None)):
+    for at, bad in ((2, -1), (2, 1 << 31), (6, 0), (6, 1 << 31), (7, 0), (7, (1 << 24) + 1), (4, 3), (10, 2 + 5), (4, 1), (5, 7), (0, None), (3, None), (9, None)):
         args = list(embed)
         args[at] = bad
         assert L.omnihd_token_embed_fwd(*args) == ARG, (at, bad)
@@ -122,7 +122,7 @@ def test_c_entries_refuse_before_any_launch():
         assert L.omnihd_block_join_bwd(*args) == status, (at, bad)
     need = L.omnihd_topk_distill_workspace_bytes(5, 8, 3, 0)
     call = [p, 0, 8, p, 0, 3, p, 1, 3, None, 5, 8, 3, 1.0, 1.0, None, None, 0, 0, p, 8, None, p, p, need, None]
-    for at, bad, status in ((24, need - 1, WORKSPACE), (23, None, ARG), (10, -1, ARG), (11, 0, ARG), (12, 0, ARG), (12, 257, ARG), (13, 0.0, ARG), (13, float("nan"), ARG), (1, 3, ARG), (4, -1, ARG),
+    for at, bad, status in ((24, need - 1, WORKSPACE), (23, None, ARG), (10, -1, ARG), (11, 0, ARG), (11, (1 << 30) + 1, ARG), (12, 0, ARG), (12, 257, ARG), (13, 0.0, ARG), (13, float("nan"), ARG), (1, 3, ARG), (4, -1, ARG),
                             (18, 1, ARG), (2, 7, ARG), (5, 2, ARG), (8, 2, ARG), (20, 7, ARG), (0, None, ARG), (3, None, ARG), (6, None, ARG)):
         args = list(call)
         args[at] = bad
