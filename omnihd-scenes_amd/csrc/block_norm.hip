@@ -147,6 +147,7 @@ template <typename TA, typename TX, int TPR, int NV, bool ODD, bool HASY>
 __global__ __launch_bounds__(threads_of<TPR>()) void k_block_bwd(BlockArgs a) {
   constexpr int TPB = threads_of<TPR>(), RPB = TPB / TPR;
   constexpr bool LEAN = NV > 1;
+  constexpr int DEPTH = TPR == 512 ? 2 : 1;         // rows asked for ahead: one block of 512 a CU has room (and need) for two
   __shared__ float red[32];
   __shared__ float fold[RPB > 1 ? TPB * 8 : 1];
   int turn = 0;
@@ -181,41 +182,39 @@ __global__ __launch_bounds__(threads_of<TPR>()) void k_block_bwd(BlockArgs a) {
 #pragma unroll
     for (int k = 0; k < 8; ++k) aw(j, k) = au(j, k) = 0.f;
   }
-  typename Raw<TX>::V xr[NV], dr[NV];
-  typename Raw<TA>::V yr[NV], hr[NV];
-  float2 stat = make_float2(1.f, 1.f);
-  auto ask = [&](long long row) {
+  struct Ahead { typename Raw<TX>::V xr[NV], dr[NV]; typename Raw<TA>::V yr[NV], hr[NV]; float2 stat; };
+  auto ask = [&](Ahead& r, long long row) {
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int c = (j * TPR + t) * 8, left = D - c;
-      xr[j] = dr[j] = typename Raw<TX>::V{};
-      yr[j] = hr[j] = typename Raw<TA>::V{};
+      r.xr[j] = r.dr[j] = typename Raw<TX>::V{};
+      r.yr[j] = r.hr[j] = typename Raw<TA>::V{};
       if (row >= hi || left <= 0) continue;
-      if (a.dh) xr[j] = raw8<ODD>(static_cast<const TX*>(a.x) + row * a.xs + c, left);
-      if (HASY) yr[j] = raw8<ODD>(static_cast<const TA*>(a.y) + row * a.ys + c, left);
-      if (HASY && a.dxo) dr[j] = raw8<ODD>(static_cast<const TX*>(a.dxo) + row * a.dxos + c, left);
-      if (a.dh) hr[j] = raw8<ODD>(static_cast<const TA*>(a.dh) + row * a.dhs + c, left);
+      if (a.dh) r.xr[j] = raw8<ODD>(static_cast<const TX*>(a.x) + row * a.xs + c, left);
+      if (HASY) r.yr[j] = raw8<ODD>(static_cast<const TA*>(a.y) + row * a.ys + c, left);
+      if (HASY && a.dxo) r.dr[j] = raw8<ODD>(static_cast<const TX*>(a.dxo) + row * a.dxos + c, left);
+      if (a.dh) r.hr[j] = raw8<ODD>(static_cast<const TA*>(a.dh) + row * a.dhs + c, left);
     }
-    if (row < hi) stat = *reinterpret_cast<const float2*>(a.stats + 2 * row);
+    r.stat = make_float2(1.f, 1.f);
+    if (row < hi) r.stat = *reinterpret_cast<const float2*>(a.stats + 2 * row);
   };
-  if (!LEAN) ask(lo + sub);
-  for (long long base = lo; base < hi; base += RPB) {
-    const long long row = base + sub;
+  // one row: what was asked for of it, and the row to ask for in its place
+  auto work = [&](Ahead& r, long long row) {
     const bool act = row < hi;
-    if (LEAN) ask(row);
-    const float ry = stat.x, rx = stat.y;
+    if (LEAN) ask(r, row);
+    const float ry = r.stat.x, rx = r.stat.y;
     float x[NV][8], y[NV][8], d[NV][8], h[NV][8], tok = 1.f;
 #pragma unroll
     for (int j = 0; j < NV; ++j)
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        x[j][k] = (float)xr[j][k];
-        y[j][k] = HASY ? (float)yr[j][k] * ry : 0.f;             // nh
-        d[j][k] = HASY ? (float)dr[j][k] : 0.f;
-        h[j][k] = (float)hr[j][k];
+        x[j][k] = (float)r.xr[j][k];
+        y[j][k] = HASY ? (float)r.yr[j][k] * ry : 0.f;             // nh
+        d[j][k] = HASY ? (float)r.dr[j][k] : 0.f;
+        h[j][k] = (float)r.hr[j][k];
       }
     if (HASY && a.gate_kind == kGateToken && act) tok = load1_any(a.gate, a.gate_type, row);
-    if (!LEAN) ask(row + RPB);
+    if (!LEAN) ask(r, row + DEPTH * RPB);
     auto row_gate = [&](int j, float (&g)[8]) {                  // what multiplies post and a gate row here: a gate of this very row
       const int c = (j * TPR + t) * 8, left = D - c;
 #pragma unroll
@@ -257,7 +256,7 @@ __global__ __launch_bounds__(threads_of<TPR>()) void k_block_bwd(BlockArgs a) {
         store8<ODD>(static_cast<TX*>(a.gx) + row * D + c, left, o);
       }
     }
-    if (!HASY) continue;
+    if (!HASY) return;
     float s = 0.f;                       // sum of t * nh * post (* gate, unless the gate is the token's): mean(m * nh), a token gate's gradient
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
@@ -293,6 +292,13 @@ __global__ __launch_bounds__(threads_of<TPR>()) void k_block_bwd(BlockArgs a) {
         store8<ODD>(static_cast<TA*>(a.gy) + row * D + c, left, o);
       }
     }
+  };
+  Ahead r0, r1;
+  if (!LEAN) ask(r0, lo + sub);
+  if (DEPTH > 1) ask(r1, lo + RPB + sub);
+  for (long long base = lo; base < hi; base += DEPTH * RPB) {
+    work(r0, base + sub);
+    if (DEPTH > 1 && base + RPB < hi) work(r1, base + RPB + sub);
   }
   if (!a.part) return;
 #pragma unroll
