@@ -151,3 +151,33 @@ def test_occupancy_head_distils(cuda):
     assert (zc.grad.double().cpu() - ref.grad).abs().max() <= 1000 * 2.0 ** -24 * ref.grad.abs().max()
     none = BEVOCCHead2Dv2.distill_loss(None, zc, t.cuda(), tid.cuda(), known=torch.zeros(shape, device="cuda"))["loss_occ_distill"]
     assert none.item() == 0
+
+
+def test_two_streams_at_once(cuda):
+    """Two training steps on two streams, work of both in flight: each as it is alone (workspaces belong to their call)."""
+    from omnihd_amd import ops
+    gen = torch.Generator().manual_seed(11)
+    sets = []
+    for k in range(2):
+        n, vocab, dim = 3000 + 500 * k, 2000, 264
+        table = torch.randn(vocab, dim, generator=gen).cuda().requires_grad_()
+        w = torch.rand(dim, generator=gen).cuda().requires_grad_()
+        y = torch.randn(n, dim, generator=gen).cuda().requires_grad_()
+        sets.append((torch.randint(0, vocab, (n,), generator=gen).cuda(), table, w, y, torch.randn(n, 5, generator=gen).cuda(), torch.randint(0, dim, (n, 5), generator=gen).cuda()))
+
+    def one(ids, table, w, y, t, tid):
+        x = ops.token_embedding(ids, table)
+        x, h = ops.block_join(x, y, post_weight=w, gate=w, next_weight=w)
+        loss = ops.topk_distill_loss(h, t, tid) + x.square().mean()
+        return [loss.detach(), *torch.autograd.grad(loss, (table, w, y))]
+    alone = [one(*s) for s in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(5):
+        got = []
+        for st, s in zip(streams, sets):
+            with torch.cuda.stream(st):
+                got.append(one(*s))
+        torch.cuda.synchronize()
+        for a, b in zip(got, alone):
+            assert all(torch.equal(u, v) for u, v in zip(a[1:], b[1:]))

@@ -260,3 +260,27 @@ def test_second_derivatives_are_refused(cuda):
     for value in (ops.topk_distill_loss(z, t, ids), ops.block_norm(z, w).sum(), ops.block_join(z, z, next_weight=w)[1].sum(), ops.token_embedding(ids, z).sum()):
         with pytest.raises(RuntimeError, match="second derivatives"):
             torch.autograd.grad(value, z, create_graph=True)
+
+
+def test_backward_captured_alone(cuda):
+    """An eager forward, its backward in a graph: every replay gives the gradient for what the upstream holds then, 1 among it."""
+    from omnihd_amd import ops
+    for vocab in (12, 700, 9000):
+        z, t, ids, _ = inputs(40, vocab, 6, F, F, vocab)
+        z.requires_grad_()
+        up = torch.ones((), device="cuda")
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            loss = ops.topk_distill_loss(z, t, ids)
+            torch.autograd.grad(ops.topk_distill_loss(z, t, ids), z, up)
+        side.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            grad, = torch.autograd.grad(loss, z, up, retain_graph=True)
+        _, _, dz, dz_terms = reference(z, t, ids, 1.0, None, 1 / 40)
+        for value in (2.0, 1.0, -3.0, 1.0):
+            up.fill_(value)
+            graph.replay()
+            torch.cuda.synchronize()
+            check_close(grad, value * dz, bound(value * dz, F, abs(value) * dz_terms, ROUNDINGS), (vocab, value))
