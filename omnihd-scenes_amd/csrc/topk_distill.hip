@@ -15,8 +15,8 @@
 // The few entries that the teacher names are written again behind the row's own stores, from their own p sums (slots with the same id are
 // summed by the first of them, so an id may stand in a row more than once).
 // Rows of up to 32 entries (the classes of a detection or occupancy head) take a lane each.
-// Measured, loss and gradient (copy rate 5.1 TB/s): 4096 x 131072 bf16 435 to 464 us (4.6 TB/s and more), 4096 x 32000 120 us (4.4), 4096 x 50001 192 us
-// (4.3), 60000 x 1000 81 us (3.1: the teacher's part of each row), 614400 x 12 fp32 30 us (2.9: 1000 instructions a wave, half of it arithmetic).
+// Measured, loss and gradient (copy rate 5.1 TB/s): 4096 x 131072 bf16 454 us (4.7 TB/s), 4096 x 32000 112 us (4.7), 4096 x 50001 188 us
+// (4.4), 60000 x 1000 70 us (3.6: the teacher's part of each row), 614400 x 12 fp32 30 us (2.9: 1000 instructions a wave, half of it arithmetic).
 #include "token_vec.h"
 
 namespace omnihd {
@@ -71,12 +71,48 @@ struct MaxNan { __device__ __forceinline__ float operator()(float a, float b) co
 // a product as it was rounded: the compiler may not take it into a fused multiply-add
 __device__ __forceinline__ float rounded(float v) { asm volatile("" : "+v"(v)); return v; }
 
+// Which of this lane's ids (bit i: slot t + i * SL) stand in the row once.  Every slot is compared with up to four of the lane's own at a
+// time: two instructions a pair (34830 rows of 172 slots: 508 us with a search for each slot).
+template <int SL, int N>
+__device__ __forceinline__ unsigned alone_of(const int* sid, int K, int at) {
+  int mine[N], seen[N];
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    mine[j] = at + j * SL < K ? sid[at + j * SL] : -2;
+    seen[j] = 0;
+  }
+#pragma unroll 4
+  for (int o = 0; o < K; ++o) {
+    const int other = sid[o];
+#pragma unroll
+    for (int j = 0; j < N; ++j) seen[j] += mine[j] == other;
+  }
+  unsigned once = 0;
+#pragma unroll
+  for (int j = 0; j < N; ++j) once |= (seen[j] == 1 ? 1u : 0u) << j;
+  return once;
+}
+template <int SL>
+__device__ __forceinline__ unsigned alone_in_row(const int* sid, int K, int t) {
+  unsigned once = 0;
+  for (int b = 0; b < K; b += 4 * SL) {
+    const int left = (K - b + SL - 1) / SL;        // (kMaxTop / 8 lanes: 32 slots a lane at most)
+    const unsigned some = left == 1 ? alone_of<SL, 1>(sid, K, b + t) : left == 2 ? alone_of<SL, 2>(sid, K, b + t)
+                        : left == 3 ? alone_of<SL, 3>(sid, K, b + t) : alone_of<SL, 4>(sid, K, b + t);
+    once |= some << (b / SL);
+  }
+  return once;
+}
+
 // TPR lanes a row; NV steps of 16 bytes a lane in registers, or (NV = 0) the row is read twice.
 template <typename T, int TPR, int NV, bool ODD>
 __global__ __launch_bounds__(TPR > 256 ? TPR : 256, TPR > 256 ? 4 : 1) void k_distill_rows(DistillArgs a) {
-  constexpr int TPB = TPR > 256 ? TPR : 256, RPB = TPB / TPR, VE = Pack<T>::n, SL = TPR < 64 ? TPR : 64, KEEP = NV ? NV : 1;
+  constexpr int TPB = TPR > 256 ? TPR : 256, RPB = TPB / TPR, VE = Pack<T>::n, KEEP = NV ? NV : 1;
+  constexpr int SL = TPR < 64 ? TPR : 64, FL = TPR > 64 ? kMaxTop : SL;      // lanes that share sums of slots, lanes with slots
+  static_assert(TPR <= 64 || TPR >= kMaxTop, "a thread a slot");
   typedef typename Pack<T>::V V;
-  __shared__ float red[32], row_coef[RPB], row_sum[RPB];
+  __shared__ float red[32], row_sum[RPB], wave_max[4], wave_sum[4], wave_part[4];
+  __shared__ bool wave_bad[4];
   extern __shared__ float slots[];       // [RPB][3][K]: ids, teacher's and student's values
   if (a.skip_if_one && *a.up == 1.f) return;
   int turn = 0;
@@ -104,37 +140,38 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256, TPR > 256 ? 4 : 1) void k_di
         }
       }
     }
-    // the teacher: lanes t < SL of the row's first wave
-    float coef = 0.f, mt = -__builtin_inff(), ls = 0.f;
-    if (TPR <= 64 || t < 64) {
-      bool bad = false;
-      if (w != 0.f)
-        for (int k = t; k < K; k += SL) {
-          const long long id = id_at(a, row * a.is + k);
-          const float v = id < 0 ? -__builtin_inff() : load1_any(a.t, a.t_type, row * a.ts + k);
-          bad |= id >= a.vocab;
-          const bool fits = id >= 0 && id < a.vocab;
-          sid[k] = fits ? (int)id : -1;
-          st[k] = v;
-          sz[k] = fits ? (float)z[id] : 0.f;
-          mt = MaxNan()(mt, v);
-        }
-      mt = lanes<SL>(mt, MaxNan());
-      bad = (bool)lanes<SL>(bad ? 1.f : 0.f, Max());
+    // The teacher.  Where a row has a block, a thread a slot, the waves' maxima and sums exchanged behind the barriers of the row's own; else
+    // the row's lanes walk over the slots.
+    float coef = 0.f, mt = -__builtin_inff(), ls = 0.f, value = -__builtin_inff();
+    bool bad = false;
+    if (t < FL && w != 0.f)
+      for (int k = t; k < K; k += FL) {
+        const long long id = id_at(a, row * a.is + k);
+        value = id < 0 ? -__builtin_inff() : load1_any(a.t, a.t_type, row * a.ts + k);
+        bad |= id >= a.vocab;
+        const bool fits = id >= 0 && id < a.vocab;
+        sid[k] = fits ? (int)id : -1;
+        st[k] = value;
+        sz[k] = fits ? (float)z[id] : 0.f;
+        mt = MaxNan()(mt, value);
+      }
+    mt = lanes<SL>(mt, MaxNan());
+    bad = (bool)lanes<SL>(bad ? 1.f : 0.f, Max());
+    if constexpr (TPR > 64) {
+      if (t < FL && (t & 63) == 0) { wave_max[t >> 6] = mt; wave_bad[t >> 6] = bad; }
+    } else {
       const bool some = w != 0.f && mt != -__builtin_inff();
       const float mtc = rounded(mt * c);
-      float s = 0.f;
+      float e = 0.f;
       if (some)
         for (int k = t; k < K; k += SL) {
           const float d = fmaf(st[k], c, -mtc);
           st[k] = d;                               // log2 of p, short of the sum's
-          s += __builtin_amdgcn_exp2f(d);
+          e += __builtin_amdgcn_exp2f(d);
         }
-      s = lanes<SL>(s, Add());
-      ls = some ? __builtin_amdgcn_logf(s) : 0.f;        // base 2
-      coef = some ? w : 0.f;
-      if (bad) coef = __builtin_nanf("");
-      if (TPR > 64 && t == 0) row_coef[sub] = coef;
+      e = lanes<SL>(e, Add());
+      ls = some ? __builtin_amdgcn_logf(e) : 0.f;        // base 2
+      coef = bad ? __builtin_nanf("") : some ? w : 0.f;
     }
     // the row's maximum and sum
     float m = -__builtin_inff(), s = 0.f, own_mc = 0.f;
@@ -174,6 +211,25 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256, TPR > 256 ? 4 : 1) void k_di
     const float own = m;
     m = group<TPR>(m, Max(), red, turn);
     const float mc = rounded(m * c);
+    bool some = false;
+    if constexpr (TPR > 64) {
+#pragma unroll
+      for (int i = 0; i < FL / 64; ++i) {
+        mt = i ? MaxNan()(mt, wave_max[i]) : wave_max[0];
+        bad = i ? bad || wave_bad[i] : wave_bad[0];
+      }
+      some = w != 0.f && mt != -__builtin_inff();
+      float e = 0.f;
+      if (some && t < FL && t < K) {
+        const float d = fmaf(value, c, -rounded(mt * c));
+        st[t] = d;
+        e = __builtin_amdgcn_exp2f(d);
+      }
+      if (t < FL) {
+        e = lanes<64>(e, Add());
+        if ((t & 63) == 0) wave_sum[t >> 6] = e;
+      }
+    }
     if (w != 0.f) {
       if constexpr (NV > 0) {
 #pragma unroll
@@ -188,7 +244,13 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256, TPR > 256 ? 4 : 1) void k_di
       }
     }
     s = group<TPR>(s, Add(), red, turn);
-    if (TPR > 64) coef = row_coef[sub];            // behind the barriers of the sums
+    if constexpr (TPR > 64) {
+      float e = wave_sum[0];
+#pragma unroll
+      for (int i = 1; i < FL / 64; ++i) e += wave_sum[i];
+      ls = some ? __builtin_amdgcn_logf(e) : 0.f;
+      coef = bad ? __builtin_nanf("") : some ? w : 0.f;
+    }
     const float scale = base * coef * a.temperature;
     float up = 1.f;
     if (a.up) up = act ? a.up[a.up_step ? row : 0] : 0.f;
@@ -228,53 +290,53 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256, TPR > 256 ? 4 : 1) void k_di
         }
       }
     }
+    const bool learns = a.g && act && k1 != 0.f;
+    unsigned alone = 0;
+    if (t < FL && learns) alone = alone_in_row<FL>(sid, K, t);
     // the teacher's entries, behind the stores of the whole row
     if (TPR > 64) __syncthreads();
     else {
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       __builtin_amdgcn_wave_barrier();
     }
-    if (TPR <= 64 || t < 64) {
-      float part = 0.f;
-      if (coef != 0.f && act) {
-        const float lq = __builtin_amdgcn_logf(s);
-        unsigned long long alone = 0;              // the lanes whose id stands in the row once: one comparison a slot tells them
-        if (SL == 64 && K <= 64) {
-          const int mine = t < K ? sid[t] : -1;
-          for (int o = 0; o < K; ++o) {
-            const unsigned long long same = __ballot(mine == __builtin_amdgcn_readlane(mine, o));
-            if ((same & (same - 1)) == 0) alone |= same;
-          }
-        }
-        for (int k = t; k < K; k += SL) {
-          const int id = sid[k];
-          if (id < 0) continue;
-          const float lp = st[k] - ls, p = __builtin_amdgcn_exp2f(lp), zk = fmaf(sz[k], c, -mc);
-          if (!(p == 0.f)) part = fmaf(p, lp - (zk - lq), part);
-          if (!a.g || k1 == 0.f) continue;
-          float sum = 0.f;                         // p of every slot with this id; only the first of them writes
-          bool leads = true;
-          if (alone >> t & 1) sum = p;
-          else
-          for (int o = 0; o < K; ++o)
-            if (sid[o] == id) {
+    float part = 0.f;
+    if (t < FL && coef != 0.f && act) {
+      const float lq = __builtin_amdgcn_logf(s);
+      for (int k = t; k < K; k += FL) {
+        const int id = sid[k];
+        if (id < 0) continue;
+        const float lp = st[k] - ls, p = __builtin_amdgcn_exp2f(lp), zk = fmaf(sz[k], c, -mc);
+        if (!(p == 0.f)) part = fmaf(p, lp - (zk - lq), part);
+        if (!learns) continue;
+        float sum = 0.f;                           // p of every slot with this id; only the first of them writes
+        bool leads = true;
+        if (alone >> ((k - t) / FL) & 1) sum = p;
+        else
+          for (int b = 0; b < K; b += 8) {         // (eight reads in flight)
+            unsigned same = 0;
+#pragma unroll
+            for (int o = 0; o < 8; ++o) same |= (b + o < K && sid[b + o < K ? b + o : 0] == id ? 1u : 0u) << o;
+            for (; same; same &= same - 1) {
+              const int o = b + __builtin_ctz(same);
               leads &= o >= k;
               sum += __builtin_amdgcn_exp2f(st[o] - ls);
             }
-          if (leads) static_cast<T*>(a.g)[row * a.gs + id] = (T)fmaf(__builtin_amdgcn_exp2f(zk), kq, -k1 * sum);
-        }
-      }
-      part = lanes<SL>(part, Add());
-      float loss = coef == 0.f ? 0.f : base * coef * a.temperature * a.temperature * kLn2 * part;
-      if (t == 0 && act) {
-        if (a.rows_out) a.rows_out[row] = loss;
-        total += loss;
+          }
+        if (leads) static_cast<T*>(a.g)[row * a.gs + id] = (T)fmaf(__builtin_amdgcn_exp2f(zk), kq, -k1 * sum);
       }
     }
-    if (TPR > 64) __syncthreads();                 // the slots are written again
+    part = lanes<SL>(part, Add());
+    if (TPR > 64 && t < FL && (t & 63) == 0) wave_part[t >> 6] = part;
+    if (TPR > 64) __syncthreads();                 // (the slots are written again)
     else {
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       __builtin_amdgcn_wave_barrier();
+    }
+    if (t == 0 && act) {
+      if constexpr (TPR > 64) part = (wave_part[0] + wave_part[1]) + (wave_part[2] + wave_part[3]);
+      const float loss = coef == 0.f ? 0.f : base * coef * a.temperature * a.temperature * kLn2 * part;
+      if (a.rows_out) a.rows_out[row] = loss;
+      total += loss;
     }
   }
   if (a.sums) {
@@ -463,7 +525,7 @@ __global__ __launch_bounds__(1024) void k_distill_total(const float* __restrict_
 
 struct Geometry { int tpr, nv; };       // nv 0: the row is read twice
 // A lane holds up to eight packs, sixteen in the longest rows.  Short rows share a wave, so that the teacher's part, much the same for any
-// vocabulary, is paid once for several (60000 x 1000 bf16: 96 us with a wave a row).
+// vocabulary, is paid once for several (60000 x 1000 bf16: 96 us with a wave a row, 70 so).
 template <typename T> Geometry geometry(int vocab, int top, bool odd) {
   const long long packs = odd ? (vocab + 2ll * (Pack<T>::n - 1)) / Pack<T>::n : vocab / Pack<T>::n;       // (odd: at any start of the row)
   int tpr = 8;

@@ -284,3 +284,19 @@ def test_backward_captured_alone(cuda):
             graph.replay()
             torch.cuda.synchronize()
             check_close(grad, value * dz, bound(value * dz, F, abs(value) * dz_terms, ROUNDINGS), (vocab, value))
+
+
+@pytest.mark.parametrize("vocab,top", [(9, 3), (30, 200), (50, 70), (300, 70), (1500, 130), (3000, 256), (6000, 256), (15000, 64), (30000, 65), (60000, 256), (120001, 200), (140000, 256)])
+def test_ids_that_stand_in_a_row_many_times(cuda, vocab, top):
+    """All slots the same, pairs side by side, pairs far apart, halves empty: an entry's gradient takes the sum of its slots."""
+    from omnihd_amd import ops
+    z, t, ids, _ = inputs(6, vocab, top, F, F, vocab + top)
+    k = torch.arange(top, device="cuda")
+    ids[0] = vocab - 1
+    ids[1] = (k // 2) % vocab
+    ids[2] = (k % max(1, top // 2)) % vocab
+    ids[3] = torch.where(k < top // 2, torch.full_like(k, 2), torch.full_like(k, -1))
+    ids[4] = torch.where(k % 3 == 0, torch.full_like(k, -7), (k * 5) % vocab)
+    for reduction in ("sum", "none"):
+        check(ops, z, t, ids, 2.0, reduction=reduction)
+    check(ops, z.bfloat16(), t, ids.int(), 2.0)
