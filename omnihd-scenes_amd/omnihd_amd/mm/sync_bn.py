@@ -37,6 +37,8 @@ class _NaiveSyncBN(nn.modules.batchnorm._BatchNorm):
 
     def forward(self, input):
         if not dist.is_available() or not dist.is_initialized() or dist.get_world_size() == 1 or not self.training:
+            if self._host_rows(input):
+                return self._forward_host_rows(input)
             return super().forward(input)
         assert input.shape[0] > 0, "SyncBN does not support empty inputs"
         from .. import ops
@@ -62,6 +64,22 @@ class _NaiveSyncBN(nn.modules.batchnorm._BatchNorm):
         bias = self.bias - mean * scale
         shape = [1, -1] + [1] * (x.dim() - 2)
         return (x * scale.reshape(shape) + bias.reshape(shape)).to(input.dtype)
+
+
+    def _host_rows(self, input):
+        return (not input.is_cuda and input.dim() == 2 and input.shape[0] > 1 and input.dtype == torch.float32 and self.training and self.affine
+                and self.track_running_stats and self.momentum is not None)
+
+    def _forward_host_rows(self, input):
+        """fp32 rows on the host (the pillar feature nets' torch formulation): batch statistics in fp64.  torch's fp32 sums over 140 000 rows go by
+        the number of host threads: 2.6e-5 of the largest output off with 16 of them, 6.6e-4 with one."""
+        mean, var = self.running_mean.double(), self.running_var.double()
+        out = nn.functional.batch_norm(input.double(), mean, var, self.weight.double(), self.bias.double(), True, self.momentum, self.eps)
+        with torch.no_grad():
+            self.running_mean.copy_(mean)
+            self.running_var.copy_(var)
+            self.num_batches_tracked.add_(1)
+        return out.to(input.dtype)
 
 
 class NaiveSyncBatchNorm1d(_NaiveSyncBN):

@@ -300,3 +300,19 @@ def test_ids_that_stand_in_a_row_many_times(cuda, vocab, top):
     for reduction in ("sum", "none"):
         check(ops, z, t, ids, 2.0, reduction=reduction)
     check(ops, z.bfloat16(), t, ids.int(), 2.0)
+
+
+@pytest.mark.parametrize("vocab,top,temperature", [(12, 4, 1.0), (40, 6, 2.0), (3000, 20, 1.0)])
+def test_differences(cuda, vocab, top, temperature):
+    """Directional derivatives by central differences.  In T^2 * ln sum exp(z / T) the third derivative along a unit-normal way is under 3 / T in
+    mean, so a step s is off by s^2 / 6 * 3 a row; the losses' rounding by 2^-24 * loss / s.  At s = 1e-2 both are under 1e-4 a row, of
+    products q * way whose absolute values sum to 0.5 and more."""
+    from omnihd_amd import ops
+    z, t, ids, gen = inputs(6, vocab, top, F, F, vocab)
+    z.requires_grad_()
+    way = torch.randn(z.shape, generator=gen).cuda()
+    value = lambda v: ops.topk_distill_loss(v, t, ids, temperature=temperature, reduction="none").double()
+    grad, = torch.autograd.grad(ops.topk_distill_loss(z, t, ids, temperature=temperature, reduction="sum"), z)
+    with torch.no_grad():
+        quotient = (value(z + 1e-2 * way) - value(z - 1e-2 * way)) / 2e-2
+    assert bool(((quotient - (grad.double() * way).sum(1)).abs() <= 2e-3).all())
