@@ -253,3 +253,50 @@ def test_stream_and_graph(cuda):
         torch.cuda.synchronize()
         now = step()
         assert all(torch.equal(now[n], held[n]) for n in now), k
+
+
+@pytest.mark.parametrize("missing", [("gate",), ("post",), ("post", "gate"), ("next",), ("gate", "next"), ("post", "gate", "next")])
+def test_single_gradients_with_missing_weights(cuda, missing):
+    """One gradient wanted, some of the weights not given: it is the one of the whole."""
+    from omnihd_amd import ops
+    x, y, pw, g, nw, gx, gh = inputs((3, 11, 88), F, F, F, "sample", True, True, 6)
+    named = {k: None if k in missing else v for k, v in dict(x=x, y=y, post=pw, gate=g, next=nw).items()}
+    whole = run_join(ops, named["x"], named["y"], named["post"], named["gate"], 0.5, named["next"], gx, gh)
+    for wanted in (k for k, v in named.items() if v is not None):
+        alone = {k: None if v is None else v.detach().requires_grad_(k == wanted) for k, v in named.items()}
+        out = ops.block_join(alone["x"], alone["y"], post_weight=alone["post"], gate=alone["gate"], residual_scale=0.5, next_weight=alone["next"], eps=EPS)
+        got, = torch.autograd.grad(out, alone[wanted], (gx, gh) if "next" not in missing else gx)
+        assert torch.equal(got, whole["g_" + wanted]), wanted
+
+
+def test_a_row_without_leading_dimensions(cuda):
+    from omnihd_amd import ops
+    x, y, pw, g, nw, gx, gh = (t[0] if t is not None and t.dim() > 1 else t for t in inputs((1, 50), B, B, F, "channel", True, True, 3))
+    a = run_join(ops, *(t.detach().requires_grad_() for t in (x, y)), pw, g, 1.0, nw, gx, gh)
+    x2, y2 = x.detach()[None].requires_grad_(), y.detach()[None].requires_grad_()
+    b = run_join(ops, x2, y2, pw, g, 1.0, nw, gx[None], gh[None])
+    for k in a:
+        assert torch.equal(a[k], b[k].reshape(a[k].shape)), k
+
+
+def test_offsets_beyond_32_bits(cuda):
+    """More than 2^31 elements: the last rows are what they are alone."""
+    from omnihd_amd import ops
+    D = 4096
+    rows = 2 ** 31 // D + 40
+    x, y = torch.zeros(rows, D, dtype=B, device="cuda"), torch.zeros(rows, D, dtype=B, device="cuda")
+    gen = torch.Generator().manual_seed(1)
+    for t in (x, y):
+        t[-50:] = torch.randn(50, D, generator=gen).bfloat16().cuda()
+    w = torch.randn(D, generator=gen).cuda()
+    gate = torch.randn(rows, 1, generator=gen).cuda()
+    up = torch.zeros(rows, D, dtype=B, device="cuda")
+    up[-50:] = torch.randn(50, D, generator=gen).bfloat16().cuda()
+    xs, ys, ws = x[-50:].clone().requires_grad_(), y[-50:].clone().requires_grad_(), w.clone().requires_grad_()
+    small = ops.block_join(xs, ys, post_weight=ws, gate=gate[-50:], next_weight=ws)
+    small_g = torch.autograd.grad(small, (xs, ys), (up[-50:], up[-50:]))
+    x.requires_grad_(), y.requires_grad_()
+    big = ops.block_join(x, y, post_weight=w, gate=gate, next_weight=w)
+    big_g = torch.autograd.grad(big, (x, y), (up, up))
+    for a, b in zip((*big, *big_g), (*small, *small_g)):
+        assert torch.equal(a[-50:], b) and not a[1000:1010].any()

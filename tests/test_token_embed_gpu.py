@@ -140,3 +140,23 @@ def test_stream_and_graph(cuda):
         torch.cuda.synchronize()
         out, grad = step()
         assert torch.equal(out, out_g) and torch.equal(grad, grad_g), k
+
+
+def test_offsets_beyond_32_bits(cuda):
+    """A table of more than 2^31 elements: rows at its end are looked up and get their gradient, every other row is zero."""
+    from omnihd_amd import ops
+    dim = 4096
+    vocab = 2 ** 31 // dim + 100
+    table = torch.zeros(vocab, dim, dtype=H, device="cuda")
+    gen = torch.Generator().manual_seed(2)
+    table[-90:] = torch.randn(90, dim, generator=gen).half().cuda()
+    table.requires_grad_()
+    ids = torch.tensor([vocab - 1, vocab - 90, 5, vocab - 1, vocab - 30], device="cuda")
+    out = ops.token_embedding(ids, table)
+    assert torch.equal(out, table.detach()[ids])
+    g = torch.randn(5, dim, generator=gen).half().cuda()
+    grad, = torch.autograd.grad(out, table, g)
+    assert torch.equal(grad[vocab - 1], (g[0].float() + g[3].float()).half())
+    assert torch.equal(grad[[vocab - 90, 5, vocab - 30]], g[[1, 2, 4]])
+    grad[[vocab - 1, vocab - 90, 5, vocab - 30]] = 0
+    assert all(not part.any() for part in grad.split(65536))

@@ -181,3 +181,21 @@ def test_two_streams_at_once(cuda):
         torch.cuda.synchronize()
         for a, b in zip(got, alone):
             assert all(torch.equal(u, v) for u, v in zip(a[1:], b[1:]))
+
+
+def test_saved_tensors_elsewhere_and_recomputed(cuda):
+    """What the operators keep for the backward may be moved to the host in between, or computed again (checkpointing): the same gradients."""
+    from torch.utils.checkpoint import checkpoint
+
+    from omnihd_amd import ops
+    p, ids, t, tid = parameters(9)
+    q = {k: v.cuda().requires_grad_() for k, v in p.items()}
+    args = (ids.cuda(), t.cuda(), tid.cuda(), torch.ones(B, L, device="cuda"))
+    want = step(ops, q, *args)
+    with torch.autograd.graph.save_on_cpu():
+        got = step(ops, q, *args)
+    for a, b in zip(got, want):
+        assert (a - b).abs().max() <= TOL * b.abs().max()
+    loss = ops.topk_distill_loss(checkpoint(lambda i: model(ops, q, i), args[0], use_reentrant=False), args[1], args[2], temperature=2.0, row_weight=args[3])
+    for a, b in zip(torch.autograd.grad(loss, list(q.values())), want[1:]):
+        assert (a - b).abs().max() <= TOL * b.abs().max()

@@ -316,3 +316,22 @@ def test_differences(cuda, vocab, top, temperature):
     with torch.no_grad():
         quotient = (value(z + 1e-2 * way) - value(z - 1e-2 * way)) / 2e-2
     assert bool(((quotient - (grad.double() * way).sum(1)).abs() <= 2e-3).all())
+
+
+def test_offsets_beyond_32_bits(cuda):
+    """More than 2^31 logits: the last rows are what they are alone."""
+    from omnihd_amd import ops
+    vocab = 131072
+    rows = 2 ** 31 // vocab + 30
+    z = torch.zeros(rows, vocab, dtype=B, device="cuda")
+    gen = torch.Generator().manual_seed(3)
+    z[-40:] = torch.randn(40, vocab, generator=gen).bfloat16().cuda()
+    t, ids = torch.randn(rows, 5, generator=gen).cuda(), torch.randint(0, vocab, (rows, 5), generator=gen).cuda()
+    small = z[-40:].clone().requires_grad_()
+    loss_s = ops.topk_distill_loss(small, t[-40:], ids[-40:], reduction="none")
+    grad_s, = torch.autograd.grad(loss_s.sum(), small)
+    z.requires_grad_()
+    loss = ops.topk_distill_loss(z, t, ids, reduction="none")
+    grad, = torch.autograd.grad(loss.sum(), z)
+    assert torch.equal(loss[-40:], loss_s) and torch.equal(grad[-40:], grad_s)
+    assert torch.allclose(grad[5].float().sum().cpu(), torch.zeros(()), atol=vocab * 2.0 ** -8 / vocab)      # q sums to 1 as p does, each rounded once
