@@ -5,10 +5,12 @@
 //
 // Both are bound by memory: rows gathered and rows written, no arithmetic to speak of.  The gradient's order of summation is fixed
 // by sorting the positions by token, without atomics on values, so it repeats bit for bit:
-//   k_embed_sort  one block per range of table rows.  Its waves each read their part of the ids: once to count what is smaller than
-//                 the range (this gives the block's place among the sorted positions) and what falls on each row of it (counters in
-//                 LDS, one set a wave), and once to put the positions in place, in order.  So the sort is one launch with no exchange
-//                 between blocks, for n ids read (rows / range) times from the L2.  Rows that got no token are zeroed here.
+//   k_embed_sort  one block per range of table rows.  Its waves each read their part of the ids, count what is smaller than the range (this
+//                 gives the block's place among the sorted positions) and what falls on each row of it (counters in LDS, one set a
+//                 wave), keep the latter, and put their positions in place, in order; where a wave has no room for them it reads its ids
+//                 again.  So the sort is one launch with no exchange between blocks, for n ids read once or twice by each of them
+//                 from the L2.  Rows that got no token are zeroed here.  Many ids go into buckets first (k_embed_count, _offsets,
+//                 _place), and each block reads its bucket's.
 //   k_embed_sum   chunks of sorted positions x column slabs: sums each run of equal tokens.  A run inside its chunk is written to the table's
 //                 gradient, a run across chunk borders as fp32 parts to the workspace: work is even however often one token occurs.
 //   k_embed_tail  joins those parts in their order.
@@ -437,8 +439,9 @@ int chunk_for(long long n, int dim) {
   while (c < 256 && (n / (2 * c)) * slabs * l >= 4096ll * 64) c *= 2;
   return c;
 }
-// From here on the ids are put into buckets first: three more launches, but no block reads all of them.
-constexpr long long kBucketIds = 1 << 17;
+// From here on the ids are put into buckets first: three more launches, but no block reads all of them (frequent-word ids, 131072 x 512: 93 us so, 84
+// without; 160000 x 256: 106 us, 143 without; 262144 x 256: 118, 201).
+constexpr long long kBucketIds = 144 << 10;
 int span_for(long long vocab) {
   const long long range = range_for(vocab), ranges = (vocab + range - 1) / range;
   return (int)(range * ((ranges + kMaxBuckets - 1) / kMaxBuckets));
@@ -470,8 +473,7 @@ BwdWs bwd_ws(long long n, long long vocab, int dim) {
 
 template <typename TT, typename TO, typename ID, bool ODD>
 int fwd(const void* ids, const void* table, long long pitch, long long vocab, long long n, int dim, float scale, void* out, hipStream_t st) {
-  // few rows: as many lanes as a row has use for; many: a wave a row at most, whose four loads a lane are in flight together
-  const int tpr = lanes_for(dim, n < 4096 ? 256 : 64);
+  const int tpr = lanes_for(dim, 256);
   const long long rpb = 256 / tpr, g = (n + rpb - 1) / rpb, most = 64ll * kMaxBlocks;
   const dim3 grid((unsigned)(g < most ? g : most)), block(256);
 #define OMNIHD_EMBED_FWD(L) hipLaunchKernelGGL((k_embed_fwd<TT, TO, ID, L, ODD>), grid, block, 0, st, static_cast<const ID*>(ids), \

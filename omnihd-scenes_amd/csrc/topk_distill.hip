@@ -14,7 +14,7 @@
 // exp2(z * c - m * c), c = log2(e) / T, one fused multiply-add with a single rounding of the difference; sums in fp32.
 // The few entries that the teacher names are written again behind the row's own stores, from their own p sums (slots with the same id are
 // summed by the first of them, so an id may stand in a row more than once).
-// Rows of up to 32 entries (the classes of a detection or occupancy head) take a lane each.
+// Rows of up to 16 entries (the classes of a detection or occupancy head) take a lane each.
 // Measured, loss and gradient (copy rate 5.1 TB/s): 4096 x 131072 bf16 454 us (4.7 TB/s), 4096 x 32000 112 us (4.7), 4096 x 50001 188 us
 // (4.4), 60000 x 1000 70 us (3.6: the teacher's part of each row), 614400 x 12 fp32 30 us (2.9: 1000 instructions a wave, half of it arithmetic).
 #include "token_vec.h"
@@ -23,7 +23,7 @@ namespace omnihd {
 namespace {
 using namespace tok;
 
-constexpr int kMaxTop = 256, kMaxVocab = 1 << 30;      // (places in a row are counted in int)
+constexpr int kLaneVocab = 16, kMaxTop = 256, kMaxVocab = 1 << 30;      // (places in a row are counted in int)
 constexpr float kLn2 = 0.69314718055994531f;
 
 struct DistillArgs {
@@ -359,7 +359,7 @@ __global__ __launch_bounds__(256) void k_distill_lanes(DistillArgs a) {
   __shared__ float wave_sum[4], staged[4][64 * PITCH];
   float* tile = staged[threadIdx.x >> 6];
   const int lane = threadIdx.x & 63;
-  const unsigned by_vocab = ((1u << 20) + a.vocab - 1) / a.vocab;          // e / vocab = e * this >> 20 for e < 64 * 32
+  const unsigned by_vocab = ((1u << 20) + a.vocab - 1) / a.vocab;          // e / vocab = e * this >> 20 for e < 64 * 16
   const bool in_dense = a.zs == a.vocab, out_dense = a.g && a.gs == a.vocab;
   if (a.skip_if_one && *a.up == 1.f) return;
   const float c = 1.44269504088896341f / a.temperature, base = factor_of(a);
@@ -539,7 +539,8 @@ template <typename T> Geometry geometry(int vocab, int top, bool odd) {
   if (packs <= 1024 * 16) return {1024, 16};
   return {1024, 0};
 }
-bool by_lanes(int vocab) { return vocab <= 32; }
+// (600000 rows of 12 entries, 4 slots: 29 us with a lane a row, 50 with eight; 300000 of 20: 34.5 and 29.6)
+bool by_lanes(int vocab) { return vocab <= kLaneVocab; }
 template <typename T> int blocks_of(long long rows, int vocab, int top, bool odd) {
   if (by_lanes(vocab)) return (int)(rows <= 16384 * 256 ? (rows + 255) / 256 : 16384);
   const int tpr = geometry<T>(vocab, top, odd).tpr, tpb = tpr > 256 ? tpr : 256;
@@ -580,8 +581,7 @@ template <typename T>
 int launch_distill(const DistillArgs& a, hipStream_t st) {
   if (by_lanes(a.vocab)) {
     const int blocks = blocks_of<T>(a.rows, a.vocab, a.top, true);
-    if (a.vocab <= 16) hipLaunchKernelGGL((k_distill_lanes<T, 16>), dim3(blocks), dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((k_distill_lanes<T, 32>), dim3(blocks), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((k_distill_lanes<T, kLaneVocab>), dim3(blocks), dim3(256), 0, st, a);
     return blocks;
   }
   auto fits = [&](const void* p, long long stride) { return !p || ((reinterpret_cast<uintptr_t>(p) & 15u) == 0 && stride % Pack<T>::n == 0); };

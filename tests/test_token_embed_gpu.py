@@ -44,8 +44,8 @@ CASES = [
     (65, 1000, 33, B, B, "order"), (1000, 50, 128, F, H, "hot"), (4100, 230000, 24, F, F, "random"), (5003, 997, 333, F, B, "runs"),
     (20011, 500, 520, B, B, "hot"), (33000, 3, 72, H, H, "same"), (9000, 20000, 1024, F, B, "order"), (777, 129, 4100, B, B, "runs"),
     (2048, 4000, 7, H, H, "hot"), (513, 600, 16, F, F, "same"), (40000, 100, 40, F, F, "runs"),
-    (131072, 5000, 16, F, F, "hot"), (140001, 3, 8, F, F, "random"), (150003, 200003, 8, F, B, "random"), (131071, 900, 9, F, F, "runs"), (200000, 700, 12, B, B, "same"),
-    (131500, 2100000, 2, F, F, "random"),
+    (131072, 5000, 16, F, F, "hot"), (147456, 3, 8, F, F, "random"), (150003, 200003, 8, F, B, "random"), (147455, 900, 9, F, F, "runs"), (200000, 700, 12, B, B, "same"),
+    (148500, 2100000, 2, F, F, "random"), (160000, 5000, 16, B, B, "hot"), (150000, 900, 9, F, F, "runs"), (300000, 40000, 8, F, F, "order"),
 ]
 
 
