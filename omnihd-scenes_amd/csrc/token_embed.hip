@@ -473,7 +473,8 @@ BwdWs bwd_ws(long long n, long long vocab, int dim) {
 
 template <typename TT, typename TO, typename ID, bool ODD>
 int fwd(const void* ids, const void* table, long long pitch, long long vocab, long long n, int dim, float scale, void* out, hipStream_t st) {
-  const int tpr = lanes_for(dim, 256);
+  // two loads a lane and row in flight: 65536 x 2048 bf16 in training 237 us a pass with two, 248 with one, 237 with four (and 64 lanes)
+  const int tpr = lanes_for((dim + 1) / 2, 256);
   const long long rpb = 256 / tpr, g = (n + rpb - 1) / rpb, most = 64ll * kMaxBlocks;
   const dim3 grid((unsigned)(g < most ? g : most)), block(256);
 #define OMNIHD_EMBED_FWD(L) hipLaunchKernelGGL((k_embed_fwd<TT, TO, ID, L, ODD>), grid, block, 0, st, static_cast<const ID*>(ids), \
