@@ -5,8 +5,10 @@
 // a training pass is bound by the host.  A pass through ctypes and a Python autograd function took 105 us (embedding), 160 us (join) on a
 // box where a bare autograd pass takes 40.  Argument checks with their messages stay in Python (omnihd_amd/ops).
 #include <torch/extension.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
 #include "omnihd_hip.h"
 
@@ -90,6 +92,16 @@ Tensor workspace(size_t bytes, const Tensor& like) { return at::empty({(int64_t)
 void no_second_order(const char* what) {
   TORCH_CHECK(!at::GradMode::is_enabled(), what, ": second derivatives (create_graph=True) are not supported");
 }
+// What follows a call by torch's own operations sees no kernel: an output would come without the tangent of a forward-mode dual tensor (its
+// directional derivative silently zero), a traced function would hold the allocation of an output and nothing that fills it.  Both are refused.
+void seen_by_autograd_alone(const char* what, std::initializer_list<Tensor> ts) {
+  namespace mode = c10::impl;
+  const bool recorded = mode::TorchDispatchModeTLS::any_modes_set() &&
+                        mode::TorchDispatchModeTLS::get_mode(mode::TorchDispatchModeKey::PROXY).has_value();
+  TORCH_CHECK_NOT_IMPLEMENTED(!recorded && !torch::jit::tracer::isTracing(), what, ": cannot be traced (torch.jit.trace, make_fx); capture a graph instead");
+  for (const Tensor& t : ts)
+    TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(0).defined(), what, ": forward-mode derivatives (dual tensors) are not supported");
+}
 Tensor of(const Maybe& t) { return t.has_value() ? *t : Tensor(); }
 bool wants_grad(std::initializer_list<Tensor> ts) {
   if (!at::GradMode::is_enabled()) return false;
@@ -140,6 +152,7 @@ struct Embed : public Function<Embed> {
 
 Tensor token_embedding(const Tensor& ids, const Tensor& table, double scale, int64_t padding, py::object out_type) {
   const auto type = torch::python::detail::py_object_to_dtype(out_type);
+  seen_by_autograd_alone("token_embedding", {table});
   const Tensor dense = ids.contiguous();
   return wants_grad({table}) ? Embed::apply(table, dense, scale, padding, (int64_t)type) : embed_forward(dense, table, scale, type);
 }
@@ -229,6 +242,7 @@ variable_list block_join(const Tensor& x, const Maybe& y, const Maybe& post, con
                          int64_t kind, int64_t per_gate, py::object act) {
   const auto type = torch::python::detail::py_object_to_dtype(act);
   const Tensor y_ = of(y), post_ = of(post), gate_ = of(gate), next_ = of(next);
+  seen_by_autograd_alone(y_.defined() ? "block_join" : "block_norm", {x, y_, post_, gate_, next_});
   if (wants_grad({x, y_, post_, gate_, next_})) return BlockJoin::apply(x, y, post, gate, next, scale, eps, kind, per_gate, (int64_t)type);
   return join_forward(x, y_, post_, gate_, next_, Join{scale, eps, kind, per_gate, type}, nullptr);
 }
@@ -294,6 +308,7 @@ struct Distill : public Function<Distill> {
 Tensor topk_distill(const Tensor& z, const Tensor& t, const Tensor& ids, const Maybe& weight, const Maybe& avg, double temperature, double factor,
                     bool per_row) {
   const Tensor teacher = t.detach(), w = of(weight), a = of(avg);
+  seen_by_autograd_alone("topk_distill_loss", {z, t, w, a});
   if (wants_grad({z})) return Distill::apply(z, teacher, ids, weight, avg, temperature, factor, per_row);
   Tensor loss;
   distill_run(z, teacher, ids, w, a, temperature, factor, per_row, &loss, Tensor(), Tensor(), false);
