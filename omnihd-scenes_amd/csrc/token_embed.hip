@@ -335,16 +335,18 @@ __global__ __launch_bounds__(256) void k_embed_sum(const TO* __restrict__ g, lon
   const int col = (int)(unit % slabs) * LANES * 8 + lane * 8, left = dim - col;
   const long long lo = c * chunk;
   if (lo >= n) return;                             // (the same in all lanes of a unit)
-  const int hi = (int)(lo + chunk < n ? lo + chunk : n);
-  const int earlier = lo > 0 ? keys[lo - 1] : -1, later = hi < n ? keys[hi] : -1;
+  const int len = (int)(lo + chunk < n ? chunk : n - lo);        // places are counted from the chunk's first: n may end at 2^31 - 1
+  const int earlier = lo > 0 ? keys[lo - 1] : -1, later = lo + len < n ? keys[lo + len] : -1;
+  keys += lo;
+  pos += lo;
   bool first = true, open = false;                 // open: the chunk's first run began in an earlier one
   float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
   auto at = [&](int v, int i) { return LANES == 64 ? __builtin_amdgcn_readlane(v, i) : __shfl(v, i, LANES); };
-  for (int b = (int)lo; b < hi; b += LANES) {
-    const int m = hi - b < LANES ? hi - b : LANES;
+  for (int b = 0; b < len; b += LANES) {
+    const int m = len - b < LANES ? len - b : LANES;
     const int mykey = lane < m ? keys[b + lane] : -1, mypos = lane < m ? pos[b + lane] : 0;
-    const int beyond = b + m < hi ? keys[b + m] : later;      // the key behind these
-    if (b == lo) open = at(mykey, 0) == earlier;
+    const int beyond = b + m < len ? keys[b + m] : later;     // the key behind these
+    if (b == 0) open = at(mykey, 0) == earlier;
     for (int i = 0; i < m; i += 8) {
       float v[8][8];
 #pragma unroll
@@ -359,7 +361,7 @@ __global__ __launch_bounds__(256) void k_embed_sum(const TO* __restrict__ g, lon
 #pragma unroll
         for (int q = 0; q < 8; ++q) acc[q] += v[k][q];
         const int key = at(mykey, i + k), next = i + k + 1 < m ? at(mykey, i + k + 1) : beyond;
-        const bool ends = b + i + k + 1 == hi;
+        const bool ends = b + i + k + 1 == len;
         if (key == next && !ends) continue;
         if ((first && open) || key == next) {      // a part of a run across chunks: its end (0) or its beginning (1)
           if (left > 0) store8<ODD>(parts + (2 * c + (first && open ? 0 : 1)) * dim + col, left, acc);

@@ -32,3 +32,17 @@ def test_forward_mode_and_traces_are_refused(cuda):
         with pytest.raises(NotImplementedError, match=f"{name}: cannot be traced"):
             torch.jit.trace(call, (x,))
         assert torch.equal(call(x), want)
+
+
+def test_embedding_gradient_of_as_many_ids_as_are_accepted(cuda):
+    """2^31 - 1 tokens of one column: the last group of eight positions ends where the next would begin beyond 2^31.  Sums of ones, whole
+    numbers under 2^24 all along, are exact in fp32 in any order."""
+    from omnihd_amd import ops
+    n, vocab = 2 ** 31 - 1, 1000
+    ids = torch.arange(n, dtype=torch.int32, device="cuda").remainder_(vocab)
+    table = torch.zeros(vocab, 1, device="cuda", requires_grad=True)
+    out = ops.token_embedding(ids, table, out_dtype=B)
+    grad, = torch.autograd.grad(out, table, torch.ones(n, 1, dtype=B, device="cuda"))
+    want = torch.full((vocab, 1), float(n // vocab), device="cuda")
+    want[:n % vocab] += 1
+    assert torch.equal(grad, want)
