@@ -32,6 +32,7 @@ struct BlockArgs {
   float *stats, *part;
   long long rows, xs, ys, gs, dxos, dhs; // row strides in elements (outputs are dense)
   long long per_gate, per_split;         // rows of one gate row, of one block
+  unsigned first;                        // backward: the launch's first block of (gate row, split)
   int splits, dim, post_type, gate_type, next_type, gate_kind, stream;
   float r, eps;
 };
@@ -142,7 +143,7 @@ __global__ __launch_bounds__(threads_of<TPR>()) void k_block_fwd(BlockArgs a) {
   }
 }
 
-// One block: `per_split` rows of one gate row (blockIdx = gate row * splits + split).  With two vectors a lane (rows beyond 8192) there are
+// One block: `per_split` rows of one gate row (unit = gate row * splits + split).  With two vectors a lane (rows beyond 8192) there are
 // not registers for all of it: the weights are read when they are used, no row is asked for ahead, and the column sums are kept in
 // LDS (128 KB) - 2048 rows of 16384 bf16: 312 us with them in registers, which spill.
 template <typename TA, typename TX, int TPR, int NV, bool ODD, bool HASY>
@@ -156,7 +157,8 @@ __global__ __launch_bounds__(threads_of<TPR>()) void k_block_bwd(BlockArgs a) {
   const int t = threadIdx.x % TPR, sub = threadIdx.x / TPR, D = a.dim;
   const float inv_d = 1.f / (float)D;
   const bool post = HASY && a.post;
-  const long long grp = blockIdx.x / a.splits, first = grp * a.per_gate, lo = first + (blockIdx.x % a.splits) * a.per_split;
+  const unsigned unit = a.first + blockIdx.x;
+  const long long grp = unit / (unsigned)a.splits, first = grp * a.per_gate, lo = first + (unit % (unsigned)a.splits) * a.per_split;
   long long hi = lo + a.per_split;
   if (hi > first + a.per_gate) hi = first + a.per_gate;
   if (hi > a.rows) hi = a.rows;
@@ -324,31 +326,42 @@ __global__ __launch_bounds__(threads_of<TPR>()) void k_block_bwd(BlockArgs a) {
             for (int k = 0; k < 8; ++k) v[k] += fold[k * TPB + o * TPR + t];
         }
       }
-      if (sub == 0 && left > 0) store8<ODD>(a.part + ((long long)blockIdx.x * 2 + which) * D + c, left, v);
+      if (sub == 0 && left > 0) store8<ODD>(a.part + ((long long)unit * 2 + which) * D + c, left, v);
     }
   }
 }
 
 // Block sums -> dnext, dpost (grp -1) and the gradient of each gate row.  16 columns by 64 places of the blocks, whose sums are joined in a
-// fixed order; four loads in flight a lane.
-__global__ __launch_bounds__(1024) void k_block_cols(const float* __restrict__ part, int blocks, int splits, int dim, const void* post,
+// fixed order; four loads in flight a lane.  Gate rows of one block sum each have nothing to join: the blocks behind the first tiles walk
+// over them, `lanes` columns at a time (there may be as many of them as rows: one block each and 16 columns would not fit a grid).
+__global__ __launch_bounds__(1024) void k_block_cols(const float* __restrict__ part, long long blocks, int splits, int dim, int lanes, const void* post,
                                                      int post_type, const void* gate, int gate_type, long long gs, int gate_kind,
                                                      void* gpost, void* ggate, void* gnext, int next_type) {
   __shared__ float s0[64][17], s1[64][17];
-  const int tiles = (dim + 15) / 16, c = (blockIdx.x % tiles) * 16 + (threadIdx.x & 15), place = threadIdx.x >> 4;
+  const int tiles = (dim + 15) / 16;
+  if (splits == 1 && (int)blockIdx.x >= tiles) {
+    const int each = 1024 / lanes;
+    for (long long grp = (long long)(blockIdx.x - tiles) * each + threadIdx.x / lanes; grp < blocks; grp += (long long)(gridDim.x - tiles) * each)
+      for (int c = threadIdx.x % lanes; c < dim; c += lanes) {
+        const float w = part[grp * 2 * dim + c];
+        store1_any(ggate, gate_type, grp * dim + c, post ? w * load1_any(post, post_type, c) : w);
+      }
+    return;
+  }
+  const int c = (blockIdx.x % tiles) * 16 + (threadIdx.x & 15), place = threadIdx.x >> 4;
   const long long grp = (long long)(blockIdx.x / tiles) - 1;
   const bool gated = gate_kind == kGateRows, many = gated && blocks > splits;
   float w = 0.f, u = 0.f;
   if (c < dim) {
     if (grp < 0) {
-      for (int b = place; b < blocks; b += 256) {
+      for (long long b = place; b < blocks; b += 256) {
         float v[4], q[4], f[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          const int i = b + 64 * k;
-          v[k] = gpost && i < blocks ? part[(long long)i * 2 * dim + c] : 0.f;
-          q[k] = gnext && i < blocks ? part[((long long)i * 2 + 1) * dim + c] : 0.f;
-          f[k] = many && gpost && i < blocks ? load1_any(gate, gate_type, (long long)(i / splits) * gs + c) : 1.f;
+          const long long i = b + 64 * k;
+          v[k] = gpost && i < blocks ? part[i * 2 * dim + c] : 0.f;
+          q[k] = gnext && i < blocks ? part[(i * 2 + 1) * dim + c] : 0.f;
+          f[k] = many && gpost && i < blocks ? load1_any(gate, gate_type, (long long)((unsigned)i / (unsigned)splits) * gs + c) : 1.f;
         }
 #pragma unroll
         for (int k = 0; k < 4; ++k) { w = fmaf(v[k], f[k], w); u += q[k]; }
@@ -393,13 +406,21 @@ void split_of(long long rows, int dim, int gate_kind, long long per_gate, bool h
   *splits = per > 0 ? (int)((per + *per_split - 1) / *per_split) : 1;
 }
 
+// A launch takes fewer than 2^32 threads
+constexpr long long most_blocks(int threads) { return 0xffffffffll / threads; }
+
 template <typename TA, typename TX, int TPR, int NV, bool ODD, bool HASY>
 void launch(const BlockArgs& a, bool bwd, long long blocks, hipStream_t st) {
   constexpr int TPB = threads_of<TPR>(), RPB = TPB / TPR;
   if (bwd) {
     const size_t wide = NV > 1 ? 2 * NV * 8 * TPB * sizeof(float) : 0;
     if (wide) (void)hipFuncSetAttribute(reinterpret_cast<const void*>(k_block_bwd<TA, TX, TPR, NV, ODD, HASY>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)wide);
-    hipLaunchKernelGGL((k_block_bwd<TA, TX, TPR, NV, ODD, HASY>), dim3((unsigned)blocks), dim3(TPB), wide, st, a);
+    constexpr long long most = most_blocks(TPB);
+    for (long long first = 0; first < blocks; first += most) {
+      BlockArgs part = a;
+      part.first = (unsigned)first;
+      hipLaunchKernelGGL((k_block_bwd<TA, TX, TPR, NV, ODD, HASY>), dim3((unsigned)(blocks - first < most ? blocks - first : most)), dim3(TPB), wide, st, part);
+    }
   } else {
     long long g = (a.rows + RPB - 1) / RPB, most = (long long)kMaxBlocks * 256 / TPB;
     const dim3 grid((unsigned)(g < most ? g : most)), block(TPB);
@@ -500,7 +521,13 @@ extern "C" int omnihd_block_join_bwd(const void* x, long long x_stride, int x_ty
   const long long blocks = groups * splits, tiles = (dim + 15) / 16;
   const bool rows_gate = gate_kind == kGateRows && g_gate;
   const bool cols = g_post || g_next || rows_gate;
-  OMNIHD_REQUIRE(blocks < (1ll << 31) && tiles * (1 + groups) < (1ll << 31), "grid");
+  // Several blocks a gate row come with fewer gate rows than blocks on the card at once (split_of): a column block for each of them and 16
+  // columns.  One block a gate row: as many column blocks as fill the card, `lanes` columns of a gate row side by side.
+  int lanes = 1;
+  while (lanes < dim && lanes < 1024) lanes *= 2;
+  const long long each = 1024 / lanes, walk = (groups + each - 1) / each;
+  const long long col_blocks = tiles + (!rows_gate ? 0 : splits > 1 ? tiles * groups : walk < kMaxBlocks ? walk : kMaxBlocks);
+  OMNIHD_REQUIRE(blocks < (1ll << 31) && col_blocks <= most_blocks(1024), "grid");
   if (rows > 0) {
     OMNIHD_REQUIRE(x && stats, "null pointer");
     if (cols) {
@@ -519,8 +546,8 @@ extern "C" int omnihd_block_join_bwd(const void* x, long long x_stride, int x_ty
     if (rc != OMNIHD_OK) return rc;
   }
   if (cols)                              // with no rows the weights' gradients are zero: no block, no gate row
-    hipLaunchKernelGGL(k_block_cols, dim3((unsigned)(tiles * (1 + (rows_gate ? groups : 0)))), dim3(1024), 0, st,
-                       static_cast<const float*>(workspace), (int)blocks, splits, dim, post, post_type, gate, gate_type, gate_stride,
+    hipLaunchKernelGGL(k_block_cols, dim3((unsigned)col_blocks), dim3(1024), 0, st,
+                       static_cast<const float*>(workspace), blocks, splits, dim, lanes, post, post_type, gate, gate_type, gate_stride,
                        gate_kind, g_post, g_gate, g_next, next_type);
   return check_launch("block_join_bwd");
 }

@@ -2,6 +2,7 @@
 import pytest
 import torch
 
+from . import test_block_norm_gpu as norm
 from .token_helpers import bound, check_close
 
 pytestmark = pytest.mark.gpu
@@ -46,3 +47,47 @@ def test_embedding_gradient_of_as_many_ids_as_are_accepted(cuda):
     want = torch.full((vocab, 1), float(n // vocab), device="cuda")
     want[:n % vocab] += 1
     assert torch.equal(grad, want)
+
+
+MANY = [
+    # samples of few rows: more gate rows than blocks on the card, fewer rows than a block has places for, one block sum or several a gate row
+    ((1500, 2, 16), F, F, F, True, True), ((700, 3, 333), B, F, F, True, True), ((300, 5, 2048), B, B, B, True, True), ((260, 2, 4100), F, F, F, True, True),
+    ((2000, 2, 8), H, H, H, False, True), ((1100, 3, 72), B, B, F, True, False), ((300, 70, 64), F, F, F, True, True), ((900, 40, 40), B, F, H, False, False),
+    ((30, 40, 2, 24), F, F, F, True, True), ((300, 2, 9001), B, B, F, True, True), ((900, 2, 1), F, F, F, True, True),
+]
+
+
+@pytest.mark.parametrize("shape,act,stream,weights,post,nxt", MANY)
+def test_many_gate_rows(cuda, shape, act, stream, weights, post, nxt):
+    from omnihd_amd import ops
+    x, y, pw, _, nw, gx, gh = norm.inputs(shape, act, stream, weights, "none", post, nxt, sum(shape))
+    gen = torch.Generator().manual_seed(sum(shape) + 1)
+    gate = (0.7 * torch.randn(*shape[:-2], 1, shape[-1], generator=gen)).to(weights).cuda().requires_grad_()
+    assert ops._gate_layout(gate, shape) == (ops._GATE_ROWS, shape[-2])
+    got = norm.run_join(ops, x, y, pw, gate, 0.75, nw, gx, gh)
+    want, terms = norm.reference(x, y, pw, gate, 0.75, nw, gx, gh)
+    norm.compare(got, want, terms, norm.rows_of(shape))
+    again = norm.run_join(ops, x, y, pw, gate, 0.75, nw, gx, gh)
+    assert all(torch.equal(got[k], again[k]) for k in got)
+
+
+@pytest.mark.parametrize("samples,rows,dim", [(16384, 4, 4096), (2 ** 24 + 5, 2, 8)])
+def test_more_gate_rows_than_one_launch_takes(cuda, samples, rows, dim):
+    """A block for each gate row and 16 columns, or for each gate row alone, would be 2^32 threads and more.  Only the first and last samples have
+    an upstream gradient, so the weights' gradients are theirs, and the samples' own are compared there."""
+    from omnihd_amd import ops
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    r = lambda *s: torch.randn(*s, generator=gen, device="cuda", dtype=B)
+    x, y, gate = r(samples, rows, dim).requires_grad_(), r(samples, rows, dim).requires_grad_(), r(samples, 1, dim).requires_grad_()
+    pw, nw = (torch.rand(dim, generator=gen, device="cuda").add_(0.5).requires_grad_() for _ in range(2))
+    assert ops._gate_layout(gate, x.shape) == (ops._GATE_ROWS, rows)
+    ends = torch.cat([torch.arange(30), torch.arange(samples - 30, samples)]).cuda()
+    gx, gh = torch.zeros_like(x), torch.zeros_like(x)
+    for g in (gx, gh):
+        g[ends] = r(60, rows, dim)
+    got = norm.run_join(ops, x, y, pw, gate, 0.75, nw, gx, gh)
+    pick = lambda t: t.detach()[ends]
+    want, terms = norm.reference(pick(x), pick(y), pw, pick(gate), 0.75, nw, pick(gx), pick(gh))
+    for k in ("g_x", "g_y", "g_gate"):
+        assert not got[k][samples // 2].any()
+    norm.compare({k: v.detach() if k in ("g_post", "g_next") else pick(v) for k, v in got.items()}, want, terms, 60 * rows)
