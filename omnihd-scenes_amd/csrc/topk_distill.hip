@@ -11,7 +11,8 @@
 // Bound by HBM at large V: V read, V written; about 15 operations an element (two exponentials among them) take half as long.  So a row
 // is read once into registers (16 bytes a lane and step), its maximum and its sum of exponentials go over the lanes that share it, and the
 // gradient is written from the registers.  Rows beyond 128 K (16-bit) entries are read twice, the second time out of the caches.  All in base 2:
-// exp2(z * c - m * c), c = log2(e) / T, one fused multiply-add with a single rounding of the difference; sums in fp32.
+// exp2(z * c - m * c), c = log2(e) / T, one fused multiply-add with a single rounding of the difference; sums in fp32.  Rows whose maximum lies far
+// from 0 are moved there first (Base).
 // The few entries that the teacher names are written again behind the row's own stores, from their own p sums (slots with the same id are
 // summed by the first of them, so an id may stand in a row more than once).
 // Rows of up to 16 entries (the classes of a detection or occupancy head) take a lane each.
@@ -70,6 +71,17 @@ struct MaxNan { __device__ __forceinline__ float operator()(float a, float b) co
 
 // a product as it was rounded: the compiler may not take it into a fused multiply-add
 __device__ __forceinline__ float rounded(float v) { asm volatile("" : "+v"(v)); return v; }
+
+// What a row's entries are shifted by: exp2(fma(v - off, c, -mc)).  The product m * c is rounded, which shifts all of them alike by half a step of it
+// and does no harm up to 2^24; beyond, the shift would leave exp2's range and masks of the type's lowest value overflow in it, so m itself is
+// taken off first (what is still in exp2's range then lies within a factor of two of m: that difference is exact).  `off` is 0 elsewhere.
+struct Base { float off, mc; };
+constexpr float kFar = 16777216.f;
+__device__ __forceinline__ Base base_of(float m, float c) {
+  const float off = fabsf(m * c) < kFar ? 0.f : m;
+  return {off, rounded((m - off) * c)};            // (NaN for a maximum that is infinite, or of a row with nothing but -inf)
+}
+__device__ __forceinline__ float below(float v, const Base& b, float c) { return fmaf(v - b.off, c, -b.mc); }
 
 // Which of this lane's ids (bit i: slot t + i * SL) stand in the row once.  Every slot is compared with up to four of the lane's own at a
 // time: two instructions a pair (34830 rows of 172 slots: 508 us with a search for each slot).
@@ -161,11 +173,11 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256, TPR > 256 ? 4 : 1) void k_di
       if (t < FL && (t & 63) == 0) { wave_max[t >> 6] = mt; wave_bad[t >> 6] = bad; }
     } else {
       const bool some = w != 0.f && mt != -__builtin_inff();
-      const float mtc = rounded(mt * c);
+      const Base tb = base_of(mt, c);
       float e = 0.f;
       if (some)
         for (int k = t; k < K; k += SL) {
-          const float d = fmaf(st[k], c, -mtc);
+          const float d = below(st[k], tb, c);
           st[k] = d;                               // log2 of p, short of the sum's
           e += __builtin_amdgcn_exp2f(d);
         }
@@ -174,7 +186,7 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256, TPR > 256 ? 4 : 1) void k_di
       coef = bad ? __builtin_nanf("") : some ? w : 0.f;
     }
     // the row's maximum and sum
-    float m = -__builtin_inff(), s = 0.f, own_mc = 0.f;
+    float m = -__builtin_inff(), s = 0.f, shift = 0.f;
     if (w != 0.f) {
       if constexpr (NV > 0) {
 #pragma unroll
@@ -194,23 +206,30 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256, TPR > 256 ? 4 : 1) void k_di
             if (at + j * TPR * VE < end)
 #pragma unroll
               for (int k = 0; k < VE; ++k) big = fmaxf(big, (float)v[j][k]);
-          if (big > m) {                           // (rescaled by the difference of the ROUNDED products that the terms are shifted by)
-            const float to = rounded(big * c);
-            s = m == -__builtin_inff() ? s : s * __builtin_amdgcn_exp2f(own_mc - to);
-            m = big;
-            own_mc = to;
+          if (big > m) {
+            s = m == -__builtin_inff() ? s : s * __builtin_amdgcn_exp2f((m - big) * c);
+            m = shift = big;                       // (shift: 0 until there is a maximum, so that -inf entries give 0)
           }
 #pragma unroll
           for (int j = 0; j < 4; ++j)
             if (at + j * TPR * VE < end)
 #pragma unroll
-              for (int k = 0; k < VE; ++k) s += __builtin_amdgcn_exp2f(fmaf((float)v[j][k], c, -own_mc));
+              for (int k = 0; k < VE; ++k) s += __builtin_amdgcn_exp2f(((float)v[j][k] - shift) * c);
         }
       }
     }
     const float own = m;
     m = group<TPR>(m, Max(), red, turn);
-    const float mc = rounded(m * c);
+    const Base zbase = NV > 0 ? base_of(m, c) : Base{m, 0.f};
+    const float mc = zbase.mc;
+    if constexpr (NV > 0) {
+      if (w != 0.f && zbase.off != 0.f)            // (the entries are this row's own from here on)
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+          if ((j * TPR + t) * VE < end)
+#pragma unroll
+            for (int k = 0; k < VE; ++k) keep[j][k] = (T)((float)keep[j][k] - zbase.off);
+    }
     bool some = false;
     if constexpr (TPR > 64) {
 #pragma unroll
@@ -221,7 +240,7 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256, TPR > 256 ? 4 : 1) void k_di
       some = w != 0.f && mt != -__builtin_inff();
       float e = 0.f;
       if (some && t < FL && t < K) {
-        const float d = fmaf(value, c, -rounded(mt * c));
+        const float d = below(value, base_of(mt, c), c);
         st[t] = d;
         e = __builtin_amdgcn_exp2f(d);
       }
@@ -240,7 +259,7 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256, TPR > 256 ? 4 : 1) void k_di
       } else if (own == -__builtin_inff()) {
         if (m == own && t * VE < end) s = __builtin_nanf("");   // nothing but -inf in the row
       } else {
-        s *= __builtin_amdgcn_exp2f(own_mc - mc);
+        s *= __builtin_amdgcn_exp2f((own - m) * c);
       }
     }
     s = group<TPR>(s, Add(), red, turn);
@@ -284,7 +303,7 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256, TPR > 256 ? 4 : 1) void k_di
             if (left <= 0) continue;
             V o;
 #pragma unroll
-            for (int k = 0; k < VE; ++k) o[k] = (T)(__builtin_amdgcn_exp2f(fmaf((float)v[j][k], c, -mc)) * kq);
+            for (int k = 0; k < VE; ++k) o[k] = (T)(__builtin_amdgcn_exp2f(((float)v[j][k] - m) * c) * kq);
             store_pack<ODD>(g + at + j * TPR * VE, left, o, skip - at - j * TPR * VE);
           }
         }
@@ -305,7 +324,7 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256, TPR > 256 ? 4 : 1) void k_di
       for (int k = t; k < K; k += FL) {
         const int id = sid[k];
         if (id < 0) continue;
-        const float lp = st[k] - ls, p = __builtin_amdgcn_exp2f(lp), zk = fmaf(sz[k], c, -mc);
+        const float lp = st[k] - ls, p = __builtin_amdgcn_exp2f(lp), zk = below(sz[k], zbase, c);
         if (!(p == 0.f)) part = fmaf(p, lp - (zk - lq), part);
         if (!learns) continue;
         float sum = 0.f;                           // p of every slot with this id; only the first of them writes
@@ -424,20 +443,27 @@ __global__ __launch_bounds__(256) void k_distill_lanes(DistillArgs a) {
     }
 #pragma unroll
     for (int k = 0; k < VM; ++k) m = fmaxf(m, x[k]);
-    const float mc = rounded(m * c);
+    float* own = tile + lane * PITCH;              // this lane's row: logits here, its gradient below
+    const Base xb = base_of(m, c);
+    const float mc = xb.mc;
+    if (xb.off != 0.f) {
+#pragma unroll
+      for (int k = 0; k < VM; ++k)
+        if (k < V_) own[k] = x[k] -= xb.off;
+    }
 #pragma unroll
     for (int k = 0; k < VM; ++k) {
       if (k < V_) { x[k] = fmaf(x[k], c, -mc); s += __builtin_amdgcn_exp2f(x[k]); }
     }
     const bool some = mt != -__builtin_inff();
-    const float mtc = rounded(mt * c);
+    const Base tb = base_of(mt, c);
     float sum = 0.f;
 #pragma unroll
-    for (int k = 0; k < KR; ++k) if (k < K) sum += __builtin_amdgcn_exp2f(fmaf(tv[k], c, -mtc));
+    for (int k = 0; k < KR; ++k) if (k < K) sum += __builtin_amdgcn_exp2f(below(tv[k], tb, c));
     for (int k = KR; k < K; ++k) {
       int i; float v;
       slot(k, i, v);
-      sum += __builtin_amdgcn_exp2f(fmaf(v, c, -mtc));
+      sum += __builtin_amdgcn_exp2f(below(v, tb, c));
     }
     float coef = w != 0.f && some ? w : 0.f;
     if (bad && w != 0.f) coef = __builtin_nanf("");
@@ -446,14 +472,13 @@ __global__ __launch_bounds__(256) void k_distill_lanes(DistillArgs a) {
     if (a.up) up = a.up[a.up_step ? row : 0];
     const float k1 = coef == 0.f ? 0.f : base * coef * a.temperature * up, kq = k1 / s;
     float part = 0.f;
-    float* own = tile + lane * PITCH;              // this lane's row: logits here, its gradient below
     auto use = [&](int i, float v) {
       if (i < 0) return;
-      const float lp = fmaf(v, c, -mtc) - ls, p = __builtin_amdgcn_exp2f(lp), zk = fmaf(own[i], c, -mc);
+      const float lp = below(v, tb, c) - ls, p = __builtin_amdgcn_exp2f(lp), zk = fmaf(own[i], c, -mc);
       if (!(p == 0.f)) part = fmaf(p, lp - (zk - lq), part);
     };
     auto learn = [&](int i, float v) {
-      if (i >= 0) own[i] -= k1 * __builtin_amdgcn_exp2f(fmaf(v, c, -mtc) - ls);
+      if (i >= 0) own[i] -= k1 * __builtin_amdgcn_exp2f(below(v, tb, c) - ls);
     };
     if (coef != 0.f) {
 #pragma unroll

@@ -3,6 +3,7 @@ import pytest
 import torch
 
 from . import test_block_norm_gpu as norm
+from . import test_topk_distill_gpu as distill
 from .token_helpers import bound, check_close
 
 pytestmark = pytest.mark.gpu
@@ -91,3 +92,31 @@ def test_more_gate_rows_than_one_launch_takes(cuda, samples, rows, dim):
     for k in ("g_x", "g_y", "g_gate"):
         assert not got[k][samples // 2].any()
     norm.compare({k: v.detach() if k in ("g_post", "g_next") else pick(v) for k, v in got.items()}, want, terms, 60 * rows)
+
+
+@pytest.mark.parametrize("vocab", [9, 12, 50, 300, 1500, 9001, 40000, 70003, 120001])
+def test_distillation_of_values_far_from_zero(cuda, vocab):
+    """Only differences count, however far from 0 the values lie: whole rows under a mask of -1e10 or of the type's lowest value, half rows, a
+    temperature of 1e-6; the teacher's slots likewise.  (A row of equal values has q = 1 / V exactly, up to the quotient's rounding.)"""
+    from omnihd_amd import ops
+    low = torch.finfo(F).min
+    z, t, ids, gen = distill.inputs(9, vocab, 5, F, F, vocab)
+    z[0], z[1], z[2, ::2], z[3, 1::2] = -1e10, low, -1e10, low
+    ids[3] -= ids[3] % 2                                   # (what the lowest value masks is not wanted: 3e38 times log2(e) is infinite)
+    z[4] = -1e10 + 1024 * torch.randint(0, 3, (vocab,), generator=gen).cuda()          # (1024: a step of fp32 there)
+    z[5] = 3e9 + 256 * torch.randint(-1, 2, (vocab,), generator=gen).cuda()
+    t[0], t[1], t[2, 1:], t[3], t[4, ::2] = -1e10, low, low, 5e9, -1e10
+    z[6], t[6] = low, low
+    for reduction in ("sum", "none"):
+        loss, grad = distill.check(ops, z, t, ids, 1.0, reduction=reduction)
+        assert bool(loss.isfinite().all() and grad.isfinite().all())
+    for far in (torch.full_like(z, 5000.0), 5000 + 2.0 ** -10 * torch.randint(0, 2, z.shape, generator=gen).cuda()):
+        loss, grad = distill.check(ops, far.float(), 3000 + 0 * t, ids, 1e-6, reduction="none")
+        assert bool(loss.isfinite().all() and grad.isfinite().all())
+    half = z.clamp(-6e4, 6e4).half()                       # a lowest value among 16-bit logits
+    half[1], half[3, 1::2] = torch.finfo(H).min, torch.finfo(H).min
+    wide = z.bfloat16()
+    wide[1], wide[3, 1::2], wide[6] = torch.finfo(B).min, torch.finfo(B).min, torch.finfo(B).min
+    for v in (half, wide):
+        loss, grad = distill.check(ops, v, t, ids, 2.0, reduction="none")
+        assert bool(loss.isfinite().all() and grad.isfinite().all())
