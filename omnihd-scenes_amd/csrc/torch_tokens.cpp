@@ -5,6 +5,7 @@
 // a training pass is bound by the host.  A pass through ctypes and a Python autograd function took 105 us (embedding), 160 us (join) on a
 // box where a bare autograd pass takes 40.  Argument checks with their messages stay in Python (omnihd_amd/ops).
 #include <torch/extension.h>
+#include <ATen/SavedTensorHooks.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
@@ -53,6 +54,8 @@ int code(const Tensor& t) { return t.scalar_type() == at::kFloat ? 0 : t.scalar_
 int code(at::ScalarType t) { return t == at::kFloat ? 0 : t == at::kBFloat16 ? 1 : 2; }
 void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 void* stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
+// tensors kept for the backward go somewhere else or are computed again (save_on_cpu, checkpointing)
+bool saved_elsewhere() { return !at::SavedTensorDefaultHooks::get_tls_state().stack.empty(); }
 bool capturing() { return c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None; }
 
 // (..., dim) as rows with one pitch between them: the tensor as it lies where the strides allow it, else a copy
@@ -268,13 +271,14 @@ void distill_run(const Tensor& z, const Tensor& t, const Tensor& ids, const Tens
 
 // The forward of a summed loss writes the logits' gradient too, while the row is in registers; the backward returns it, after a launch that
 // writes it again where the gradient arriving at the loss is not 1.  That second form alone (two passes instead of one and a half) serves
-// per-row losses, whose upstream gradient is not known in the forward, stream capture, whose replays may be of the backward alone, and
-// every further backward pass over the same forward.
+// per-row losses, whose upstream gradient is not known in the forward, stream capture, whose replays may be of the backward alone,
+// every further backward pass over the same forward, and forwards under saved-tensor hooks: the gradient is no saved tensor, so that the hooks could
+// not take it off the device, and one of the logits' size would be held from the forward that they are meant to relieve.
 struct Distill : public Function<Distill> {
   static Tensor forward(AutogradContext* ctx, Tensor z, Tensor t, Tensor ids, Maybe weight_, Maybe avg_, double temperature, double factor,
                         bool per_row) {
     const Tensor weight = of(weight_), avg = of(avg_);
-    const bool fresh = !per_row && !capturing();
+    const bool fresh = !per_row && !saved_elsewhere() && !capturing();
     Tensor loss, grad;
     if (fresh) grad = dense_like(z);
     distill_run(z, t, ids, weight, avg, temperature, factor, per_row, &loss, grad, Tensor(), false);
@@ -290,13 +294,12 @@ struct Distill : public Function<Distill> {
     const variable_list in = ctx->get_saved_variables();
     Tensor grad;
     const auto kept = ctx->saved_data.find("grad");
-    const bool in_place = kept != ctx->saved_data.end() && !capturing();
-    if (in_place) {
-      grad = kept->second.toTensor();
-      ctx->saved_data.erase(kept);
-    } else {
-      grad = dense_like(in[0]);
+    if (kept != ctx->saved_data.end()) {
+      if (!capturing()) grad = kept->second.toTensor();
+      ctx->saved_data.erase(kept);                  // (a captured backward has no use for it)
     }
+    const bool in_place = grad.defined();
+    if (!in_place) grad = dense_like(in[0]);
     distill_run(in[0], in[1], in[2], in[3], in[4], ctx->saved_data["temperature"].toDouble(), ctx->saved_data["factor"].toDouble(),
                 ctx->saved_data["per_row"].toBool(), nullptr, grad, ups[0].contiguous(), in_place);
     variable_list grads(8);

@@ -120,3 +120,61 @@ def test_distillation_of_values_far_from_zero(cuda, vocab):
     for v in (half, wide):
         loss, grad = distill.check(ops, v, t, ids, 2.0, reduction="none")
         assert bool(loss.isfinite().all() and grad.isfinite().all())
+
+
+def test_distillation_holds_no_gradient_that_hooks_or_capture_do_not_see(cuda):
+    """Device memory of a summed loss between forward and backward: one gradient beside the logits in a plain step, none where saved tensors go
+    elsewhere or are computed again, none once its backward is captured; values and gradients are the same bits everywhere."""
+    from torch.utils.checkpoint import checkpoint
+
+    from omnihd_amd import ops
+    rows, vocab = 512, 32000
+    size, small = rows * vocab * 4, 4 << 20
+    z, t, ids, _ = distill.inputs(rows, vocab, 6, F, F, 1)
+    z.requires_grad_()
+    call = lambda v: ops.topk_distill_loss(v, t, ids, temperature=2.0)
+    want, = torch.autograd.grad(call(z), z)
+    value = call(z.detach())
+
+    def held(forward):
+        torch.cuda.synchronize()
+        before = torch.cuda.memory_allocated()
+        loss = forward()
+        between = torch.cuda.memory_allocated() - before
+        torch.cuda.reset_peak_memory_stats()
+        grad, = torch.autograd.grad(loss, z)
+        peak = torch.cuda.max_memory_allocated() - before
+        assert torch.equal(loss, value) and torch.equal(grad, want)
+        return between, peak
+
+    def moved():
+        with torch.autograd.graph.saved_tensors_hooks(lambda v: v, lambda v: v):
+            return call(z)
+    between, peak = held(lambda: call(z))
+    assert size <= between < size + small and peak < size + small
+    for forward in (lambda: checkpoint(call, z, use_reentrant=False), moved):
+        between, peak = held(forward)
+        assert between < small and peak < size + small
+    with torch.autograd.graph.save_on_cpu():
+        loss = call(z)
+    grad, = torch.autograd.grad(loss, z)
+    assert torch.equal(grad, want)
+    del loss, grad
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    up = torch.ones((), device="cuda")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        loss = call(z)
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        grad, = torch.autograd.grad(loss, z, up, retain_graph=True)
+    assert torch.cuda.memory_allocated() - before < size + small           # the captured backward's own
+    for factor in (1.0, 2.0, 1.0):
+        up.fill_(factor)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(grad, factor * want)
+        assert torch.equal(torch.autograd.grad(loss, z, up, retain_graph=True)[0], grad)
