@@ -278,6 +278,7 @@ struct Distill : public Function<Distill> {
   static Tensor forward(AutogradContext* ctx, Tensor z, Tensor t, Tensor ids, Maybe weight_, Maybe avg_, double temperature, double factor,
                         bool per_row) {
     const Tensor weight = of(weight_), avg = of(avg_);
+    c10::DeviceGuard guard(z.device());             // (whether a stream is captured is asked of the logits' device)
     const bool fresh = !per_row && !saved_elsewhere() && !capturing();
     Tensor loss, grad;
     if (fresh) grad = dense_like(z);

@@ -178,3 +178,28 @@ def test_distillation_holds_no_gradient_that_hooks_or_capture_do_not_see(cuda):
         torch.cuda.synchronize()
         assert torch.equal(grad, factor * want)
         assert torch.equal(torch.autograd.grad(loss, z, up, retain_graph=True)[0], grad)
+
+
+@pytest.mark.skipif(torch.cuda.device_count() < 2, reason="asks for the state of a second device's stream")
+def test_capture_on_another_device_than_the_current_one(cuda):
+    """The forward captured on the logits' device while another one is current: every replay's gradient follows the logits."""
+    from omnihd_amd import ops
+    other = torch.device("cuda:1")
+    z, t, ids = (v.to(other) for v in distill.inputs(20, 900, 6, F, F, 1)[:3])
+    z.requires_grad_()
+
+    def step():
+        with torch.cuda.device(0):
+            return torch.autograd.grad(ops.topk_distill_loss(z, t, ids), z)[0]
+    with torch.cuda.device(other):
+        step()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            held = step()
+        for _ in range(3):
+            with torch.no_grad():
+                z.normal_()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(held, step())
