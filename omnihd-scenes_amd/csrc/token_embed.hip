@@ -581,6 +581,7 @@ extern "C" int omnihd_token_embed_bwd(const void* ids, int wide_ids, long long n
                                       void* workspace, size_t workspace_bytes, void* stream) {
   OMNIHD_EMBED_CHECKS;
   OMNIHD_REQUIRE(grad && workspace && (n == 0 || (ids && g && g_stride >= dim)), "null pointer or short rows");
+  if (padding >= vocab) padding = -1;              // no row of the table (ids are compared as 32 bits below)
   const BwdWs at = bwd_ws(n, vocab, dim);
   if (workspace_bytes < at.total) { set_error("token_embed_bwd: workspace %zu < required %zu", workspace_bytes, at.total); return OMNIHD_ERR_WORKSPACE; }
   OMNIHD_REQUIRE(at.chunks * ((dim + 63) / 64) < (1ll << 31), "grid");

@@ -203,3 +203,20 @@ def test_capture_on_another_device_than_the_current_one(cuda):
             graph.replay()
             torch.cuda.synchronize()
             assert torch.equal(held, step())
+
+
+@pytest.mark.parametrize("n", [50, 150000])
+@pytest.mark.parametrize("padding", [-1, 40, 2 ** 31 - 1, 2 ** 32 + 3, 2 ** 40 + 3, -2 ** 32 + 3, 3])
+def test_padding_outside_the_table(cuda, n, padding):
+    """At the C entry, which takes 64 bits: only a row of the table is left out."""
+    from omnihd_amd._lib import lib
+    L, vocab, dim = lib(), 40, 8
+    ids = torch.arange(n, device="cuda") % vocab
+    g, grad = torch.ones(n, dim, device="cuda"), torch.empty(vocab, dim, device="cuda")
+    ws = torch.empty(L.omnihd_token_embed_bwd_workspace_bytes(n, vocab, dim), dtype=torch.uint8, device="cuda")
+    assert L.omnihd_token_embed_bwd(ids.data_ptr(), 1, n, g.data_ptr(), 0, dim, vocab, dim, 1.0, padding, grad.data_ptr(), 0, ws.data_ptr(), ws.numel(),
+                                    torch.cuda.current_stream().cuda_stream) == 0
+    want = torch.bincount(ids, minlength=vocab).float()
+    if 0 <= padding < vocab:
+        want[padding] = 0
+    assert torch.equal(grad, want[:, None].expand(vocab, dim))
