@@ -18,7 +18,7 @@ replace functions through it); state that code REBINDS lives in one part and is 
 from . import _core
 from ._core import (_ptr, _current_device, _raw_stream, _stream, _want, _same_device, _workspace, _NULL_CTX, _SIZE_CACHE, _on,
     _WGRAD_WS, _wgrad_workspace, _want_cl, _pair_same, deterministic, FAST_PATHS, _CL, _rows_view, _f32c,
-    _ROW_TYPES, _want_rows)
+    _ROW_TYPES, _want_rows, _constant)
 from . import pool
 from .pool import (bev_pool_v2_forward, bev_pool_v2_backward, bev_pool_v2_forward_csr, _PREFETCH_STREAMS, prefetch,
     bev_pool_v2_forward_direct, bev_pool_v2_backward_patch, tile_descriptors, csr_tiles, _nhwc_rows, _DepthHead,

@@ -132,3 +132,12 @@ def _want_rows(t, name):
         raise RuntimeError(f"{name} must be a CUDA(HIP) tensor; the HIP ops have no CPU path")
     if t.dtype not in _ROW_TYPES:
         raise TypeError(f"{name} must be float32, bfloat16 or float16, got {t.dtype}")
+
+
+def _constant(value, name):
+    """A number that a kernel takes by value.  A tensor that wants a gradient (or carries a tangent) would be taken for one without a word."""
+    if isinstance(value, torch.Tensor):
+        wants = torch.is_grad_enabled() and value.requires_grad
+        if wants or torch.autograd.forward_ad.unpack_dual(value).tangent is not None:
+            raise TypeError(f"{name} is a constant of the operator and gets no gradient: give a number, or multiply outside")
+    return float(value)

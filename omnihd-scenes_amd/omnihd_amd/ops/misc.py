@@ -12,7 +12,7 @@ import torch
 
 from .._env import env as _env
 from .._lib import check, lib, torch_ops
-from ._core import _ROW_TYPES, _on, _ptr, _raw_stream, _same_device, _stream, _want, _want_rows, _workspace
+from ._core import _ROW_TYPES, _constant, _on, _ptr, _raw_stream, _same_device, _stream, _want, _want_rows, _workspace
 
 
 
@@ -196,7 +196,7 @@ def token_embedding(ids, table, scale=1.0, padding_idx=None, out_dtype=None):
         if not -table.shape[0] <= padding_idx < table.shape[0]:
             raise ValueError(f"padding_idx {padding_idx} is not a row of a table of {table.shape[0]}")
         padding = int(padding_idx) % table.shape[0]
-    return torch_ops().token_embedding(ids, table, scale, padding, out_dtype)
+    return torch_ops().token_embedding(ids, table, _constant(scale, "scale"), padding, out_dtype)
 
 
 # --------------------------------------------------------------------------------------------
@@ -229,7 +229,7 @@ def topk_distill_loss(logits, teacher_logits, teacher_ids, temperature=1.0, row_
         raise ValueError(f"teacher_logits and teacher_ids must be {lead} + (K,), got {tuple(teacher_logits.shape)} and {tuple(teacher_ids.shape)}")
     if not 1 <= teacher_ids.shape[-1] <= _DISTILL_MAX_TOP:
         raise ValueError(f"1 to {_DISTILL_MAX_TOP} kept entries a row are supported, got {teacher_ids.shape[-1]}")
-    temperature, loss_weight = float(temperature), float(loss_weight)
+    temperature, loss_weight = _constant(temperature, "temperature"), _constant(loss_weight, "loss_weight")
     if not 1e-6 <= temperature <= 1e6:
         raise ValueError(f"temperature must be in [1e-6, 1e6], got {temperature}")
     if reduction not in ("mean", "sum", "none"):

@@ -12,7 +12,7 @@ import torch
 
 from .._env import env as _env
 from .._lib import check, lib, torch_ops
-from ._core import (FAST_PATHS, _ROW_TYPES, _SIZE_CACHE, _f32c, _on, _raw_stream, _rows_view, _same_device, _want, _want_rows,
+from ._core import (FAST_PATHS, _ROW_TYPES, _SIZE_CACHE, _constant, _f32c, _on, _raw_stream, _rows_view, _same_device, _want, _want_rows,
     _wgrad_workspace)
 from .policy import _fp32_policy, f16_handover
 from .planes import _alloc_planes, _amax_slot, half_wanted, planes_wanted, tag_half, tag_planes, tag_producer
@@ -288,7 +288,9 @@ def _gate_layout(gate, shape):
 
 
 def _block_checks(x, eps, *weights):
+    """Raises for what the block norms do not take; eps as a number."""
     _want_rows(x, "x")
+    eps = _constant(eps, "eps")
     if not 1 <= x.shape[-1] <= _BLOCK_MAX_DIM:
         raise ValueError(f"rows of {x.shape[-1]} elements: 1 to {_BLOCK_MAX_DIM} are supported")
     if not eps >= 1e-30:
@@ -299,13 +301,14 @@ def _block_checks(x, eps, *weights):
             if tuple(w.shape) != (x.shape[-1],):
                 raise ValueError(f"{name} must have shape ({x.shape[-1]},), got {tuple(w.shape)}")
             _same_device(x, w)
+    return eps
 
 
 def block_norm(x, weight, eps=1e-6, out_dtype=None):
     """The norm in front of a block: ``x * rsqrt(mean(x^2) + eps) * weight`` over the last dimension (up to 16384), x (..., D) fp32, bf16 or
     fp16, weight (D,) of any of these types; ``out_dtype``: x's (the default), or a 16-bit type for an fp32 x.  Differentiable in both.
     See ``block_join`` for the norms behind it."""
-    _block_checks(x, eps, (weight, "weight"))
+    eps = _block_checks(x, eps, (weight, "weight"))
     if weight is None:
         raise TypeError("weight must be a tensor")
     act = x.dtype if out_dtype is None else out_dtype
@@ -324,7 +327,7 @@ def block_join(x, y, post_weight=None, gate=None, residual_scale=1.0, next_weigh
     fp32 value of x_out, before its rounding).  gate: (D,), or the leading dimensions of x with ones behind and D (one row a sample), or
     (..., 1) (a number a row), or y's shape; weights and gate fp32, bf16 or fp16, D up to 16384.  Returns x_out, or (x_out, h) with next_weight.
     Differentiable in all five, sums over rows in a fixed order; a single token is a row like any other."""
-    _block_checks(x, eps, (post_weight, "post_weight"), (next_weight, "next_weight"))
+    eps = _block_checks(x, eps, (post_weight, "post_weight"), (next_weight, "next_weight"))
     _want_rows(y, "y")
     if y.shape != x.shape:
         raise ValueError(f"y must have x's shape {tuple(x.shape)}, got {tuple(y.shape)}")
@@ -335,5 +338,5 @@ def block_join(x, y, post_weight=None, gate=None, residual_scale=1.0, next_weigh
     if gate is not None:
         _want_rows(gate, "gate")
         kind, per_gate = _gate_layout(gate, tuple(x.shape))
-    got = torch_ops().block_join(x, y, post_weight, gate, next_weight, residual_scale, eps, kind, per_gate, y.dtype)
+    got = torch_ops().block_join(x, y, post_weight, gate, next_weight, _constant(residual_scale, "residual_scale"), eps, kind, per_gate, y.dtype)
     return got[0] if next_weight is None else tuple(got)

@@ -51,3 +51,41 @@ def test_traces_are_refused(call, name):
         torch.jit.trace(body, (m[name],))
     with pytest.raises(NotImplementedError, match=f"{call}: cannot be traced"):
         make_fx(body)(m[name])
+
+
+class OnDevice(torch.Tensor):
+    """A CPU tensor that says it is on the GPU: the wrappers' argument checks run on it."""
+    is_cuda = True
+
+
+def test_numbers_that_want_a_gradient_are_refused(monkeypatch):
+    """They would be taken for constants; under no_grad, and as numbers or plain tensors, they are what they were."""
+    from omnihd_amd import ops
+    from omnihd_amd.ops import misc, norm
+    seen = []
+
+    class Face:
+        def __getattr__(self, name):
+            return lambda *args: (seen.append([a for a in args if type(a) is float]), [None, None])[1]
+    monkeypatch.setattr(misc, "torch_ops", Face)
+    monkeypatch.setattr(norm, "torch_ops", Face)
+    m = {k: v.as_subclass(OnDevice) for k, v in tensors().items()}
+    ids = torch.zeros(ROWS, TOP, dtype=torch.int64).as_subclass(OnDevice)
+    calls = {
+        "scale": lambda v: ops.token_embedding(ids, m["table"], scale=v), "eps": lambda v: ops.block_norm(m["x"], m["next"], eps=v),
+        "residual_scale": lambda v: ops.block_join(m["x"], m["y"], residual_scale=v), "temperature": lambda v: ops.topk_distill_loss(m["z"], m["t"], ids, temperature=v),
+        "loss_weight": lambda v: ops.topk_distill_loss(m["z"], m["t"], ids, loss_weight=v, reduction="sum"),
+    }
+    for name, call in calls.items():
+        learnt = torch.tensor(0.5, requires_grad=True)
+        with pytest.raises(TypeError, match=f"{name} is a constant"):
+            call(learnt)
+        with fw.dual_level(), pytest.raises(TypeError, match=f"{name} is a constant"):
+            call(fw.make_dual(torch.tensor(0.5), torch.tensor(1.0)))
+        assert not seen
+        with torch.no_grad():
+            call(learnt)
+        for value in (0.5, torch.tensor(0.5), torch.tensor([0.5])):
+            call(value)
+        assert len(seen) == 4 and all(0.5 in floats for floats in seen)
+        seen.clear()
