@@ -220,3 +220,28 @@ def test_padding_outside_the_table(cuda, n, padding):
     if 0 <= padding < vocab:
         want[padding] = 0
     assert torch.equal(grad, want[:, None].expand(vocab, dim))
+
+
+@pytest.mark.parametrize("amp", [False, True])
+def test_occupancy_head_trains_from_a_teacher(cuda, amp):
+    """The built head, from features to its parameters' gradients, with a teacher head's best four classes a voxel: the loss's own gradient against the
+    definition, and every parameter gets what the head passes on of it."""
+    from omnihd_amd.mm.registry import HEADS, build_from_cfg
+    from projects.mmdet3d_plugin.bevfusion.dense_heads import bev_occ_head  # noqa: F401
+    cfg = dict(type="BEVOCCHead2Dv2", in_dim=16, out_dim=16, Dz=4, num_classes=12, loss_occ=dict(type="CrossEntropyLoss", ignore_index=255, loss_weight=1.0))
+    student, teacher = (build_from_cfg(cfg, HEADS).cuda() for _ in range(2))
+    feats = torch.randn(2, 16, 6, 5, device="cuda")
+    with torch.no_grad():
+        t, tid = teacher([feats]).mul(3).topk(4, -1)
+    known = torch.rand(t.shape[:-1], device="cuda") < 0.7
+    with torch.autocast("cuda", torch.bfloat16, enabled=amp):
+        pred = student([feats])
+    assert pred.shape == (2, 5, 6, 4, 12) and pred.dtype == (B if amp else F)
+    loss = student.distill_loss(pred, t, tid, known=known, temperature=1.5, loss_weight=0.5)["loss_occ_distill"]
+    grad, = torch.autograd.grad(loss, pred, retain_graph=True)
+    flat = lambda v: v.reshape(-1, v.shape[-1])
+    count = float(known.sum())
+    _, _, dz, terms = distill.reference(flat(pred), flat(t), flat(tid), 1.5, known.reshape(-1).float(), 0.5 / count)
+    check_close(flat(grad), dz, bound(dz, pred.dtype, terms, distill.ROUNDINGS), "gradient")
+    for g in torch.autograd.grad(loss, list(student.parameters())):
+        assert bool(g.isfinite().all()) and bool(g.any())
