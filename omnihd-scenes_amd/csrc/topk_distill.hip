@@ -74,7 +74,8 @@ __device__ __forceinline__ float rounded(float v) { asm volatile("" : "+v"(v)); 
 
 // What a row's entries are shifted by: exp2(fma(v - off, c, -mc)).  The product m * c is rounded, which shifts all of them alike by half a step of it
 // and does no harm up to 2^24; beyond, the shift would leave exp2's range and masks of the type's lowest value overflow in it, so m itself is
-// taken off first (what is still in exp2's range then lies within a factor of two of m: that difference is exact).  `off` is 0 elsewhere.
+// taken off first (what is still in exp2's range then lies within a factor of two of m: that difference is exact, in the entries' own type too).
+// `off` is 0 elsewhere, and the entries are moved in a branch of their own: a subtraction for every one of them costs 17 % at 614400 x 12.
 struct Base { float off, mc; };
 constexpr float kFar = 16777216.f;
 __device__ __forceinline__ Base base_of(float m, float c) {
@@ -82,6 +83,12 @@ __device__ __forceinline__ Base base_of(float m, float c) {
   return {off, rounded((m - off) * c)};            // (NaN for a maximum that is infinite, or of a row with nothing but -inf)
 }
 __device__ __forceinline__ float below(float v, const Base& b, float c) { return fmaf(v - b.off, c, -b.mc); }
+// how far one shift lies below another
+__device__ __forceinline__ float between(const Base& a, const Base& b, float c) { return fmaf(a.off - b.off, c, a.mc - b.mc); }
+template <typename T> __device__ __forceinline__ void move(typename Pack<T>::V& v, float off) {
+#pragma unroll
+  for (int k = 0; k < Pack<T>::n; ++k) v[k] = (T)((float)v[k] - off);
+}
 
 // Which of this lane's ids (bit i: slot t + i * SL) stand in the row once.  Every slot is compared with up to four of the lane's own at a
 // time: two instructions a pair (34830 rows of 172 slots: 508 us with a search for each slot).
@@ -186,7 +193,8 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256, TPR > 256 ? 4 : 1) void k_di
       coef = bad ? __builtin_nanf("") : some ? w : 0.f;
     }
     // the row's maximum and sum
-    float m = -__builtin_inff(), s = 0.f, shift = 0.f;
+    float m = -__builtin_inff(), s = 0.f;
+    Base at_base{0.f, 0.f};                        // what this lane's terms are shifted by so far (rows read twice)
     if (w != 0.f) {
       if constexpr (NV > 0) {
 #pragma unroll
@@ -207,28 +215,32 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256, TPR > 256 ? 4 : 1) void k_di
 #pragma unroll
               for (int k = 0; k < VE; ++k) big = fmaxf(big, (float)v[j][k]);
           if (big > m) {
-            s = m == -__builtin_inff() ? s : s * __builtin_amdgcn_exp2f((m - big) * c);
-            m = shift = big;                       // (shift: 0 until there is a maximum, so that -inf entries give 0)
+            const Base to = base_of(big, c);
+            s = m == -__builtin_inff() ? s : s * __builtin_amdgcn_exp2f(between(at_base, to, c));
+            m = big;
+            at_base = to;
           }
+          if (at_base.off != 0.f)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (at + j * TPR * VE < end) move<T>(v[j], at_base.off);
 #pragma unroll
           for (int j = 0; j < 4; ++j)
             if (at + j * TPR * VE < end)
 #pragma unroll
-              for (int k = 0; k < VE; ++k) s += __builtin_amdgcn_exp2f(((float)v[j][k] - shift) * c);
+              for (int k = 0; k < VE; ++k) s += __builtin_amdgcn_exp2f(fmaf((float)v[j][k], c, -at_base.mc));
         }
       }
     }
     const float own = m;
     m = group<TPR>(m, Max(), red, turn);
-    const Base zbase = NV > 0 ? base_of(m, c) : Base{m, 0.f};
+    const Base zbase = base_of(m, c);
     const float mc = zbase.mc;
     if constexpr (NV > 0) {
-      if (w != 0.f && zbase.off != 0.f)            // (the entries are this row's own from here on)
+      if (w != 0.f && zbase.off != 0.f)
 #pragma unroll
         for (int j = 0; j < NV; ++j)
-          if ((j * TPR + t) * VE < end)
-#pragma unroll
-            for (int k = 0; k < VE; ++k) keep[j][k] = (T)((float)keep[j][k] - zbase.off);
+          if ((j * TPR + t) * VE < end) move<T>(keep[j], zbase.off);
     }
     bool some = false;
     if constexpr (TPR > 64) {
@@ -259,7 +271,7 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256, TPR > 256 ? 4 : 1) void k_di
       } else if (own == -__builtin_inff()) {
         if (m == own && t * VE < end) s = __builtin_nanf("");   // nothing but -inf in the row
       } else {
-        s *= __builtin_amdgcn_exp2f((own - m) * c);
+        s *= __builtin_amdgcn_exp2f(between(at_base, zbase, c));
       }
     }
     s = group<TPR>(s, Add(), red, turn);
@@ -301,9 +313,10 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256, TPR > 256 ? 4 : 1) void k_di
           for (int j = 0; j < 4; ++j) {
             const int left = end - at - j * TPR * VE;
             if (left <= 0) continue;
+            if (zbase.off != 0.f) move<T>(v[j], zbase.off);
             V o;
 #pragma unroll
-            for (int k = 0; k < VE; ++k) o[k] = (T)(__builtin_amdgcn_exp2f(((float)v[j][k] - m) * c) * kq);
+            for (int k = 0; k < VE; ++k) o[k] = (T)(__builtin_amdgcn_exp2f(fmaf((float)v[j][k], c, -mc)) * kq);
             store_pack<ODD>(g + at + j * TPR * VE, left, o, skip - at - j * TPR * VE);
           }
         }
@@ -457,9 +470,13 @@ __global__ __launch_bounds__(256) void k_distill_lanes(DistillArgs a) {
     }
     const bool some = mt != -__builtin_inff();
     const Base tb = base_of(mt, c);
+    if (tb.off != 0.f) {
+#pragma unroll
+      for (int k = 0; k < KR; ++k) tv[k] -= tb.off;
+    }
     float sum = 0.f;
 #pragma unroll
-    for (int k = 0; k < KR; ++k) if (k < K) sum += __builtin_amdgcn_exp2f(below(tv[k], tb, c));
+    for (int k = 0; k < KR; ++k) if (k < K) sum += __builtin_amdgcn_exp2f(fmaf(tv[k], c, -tb.mc));
     for (int k = KR; k < K; ++k) {
       int i; float v;
       slot(k, i, v);
@@ -472,21 +489,21 @@ __global__ __launch_bounds__(256) void k_distill_lanes(DistillArgs a) {
     if (a.up) up = a.up[a.up_step ? row : 0];
     const float k1 = coef == 0.f ? 0.f : base * coef * a.temperature * up, kq = k1 / s;
     float part = 0.f;
-    auto use = [&](int i, float v) {
+    auto use = [&](int i, float d) {               // (d: below(value, tb, c))
       if (i < 0) return;
-      const float lp = below(v, tb, c) - ls, p = __builtin_amdgcn_exp2f(lp), zk = fmaf(own[i], c, -mc);
+      const float lp = d - ls, p = __builtin_amdgcn_exp2f(lp), zk = fmaf(own[i], c, -mc);
       if (!(p == 0.f)) part = fmaf(p, lp - (zk - lq), part);
     };
-    auto learn = [&](int i, float v) {
-      if (i >= 0) own[i] -= k1 * __builtin_amdgcn_exp2f(below(v, tb, c) - ls);
+    auto learn = [&](int i, float d) {
+      if (i >= 0) own[i] -= k1 * __builtin_amdgcn_exp2f(d - ls);
     };
     if (coef != 0.f) {
 #pragma unroll
-      for (int k = 0; k < KR; ++k) if (k < K) use(id[k], tv[k]);
+      for (int k = 0; k < KR; ++k) if (k < K) use(id[k], fmaf(tv[k], c, -tb.mc));
       for (int k = KR; k < K; ++k) {
         int i; float v;
         slot(k, i, v);
-        use(i, v);
+        use(i, below(v, tb, c));
       }
     }
     if (a.g) {
@@ -496,11 +513,11 @@ __global__ __launch_bounds__(256) void k_distill_lanes(DistillArgs a) {
         if (k < V_) own[k] = k1 == 0.f ? 0.f : __builtin_amdgcn_exp2f(x[k]) * kq;
       if (k1 != 0.f) {
 #pragma unroll
-        for (int k = 0; k < KR; ++k) if (k < K) learn(id[k], tv[k]);
+        for (int k = 0; k < KR; ++k) if (k < K) learn(id[k], fmaf(tv[k], c, -tb.mc));
         for (int k = KR; k < K; ++k) {
           int i; float v;
           slot(k, i, v);
-          learn(i, v);
+          learn(i, below(v, tb, c));
         }
       }
       if (!out_dense && act) {

@@ -136,6 +136,8 @@ def _want_rows(t, name):
 
 def _constant(value, name):
     """A number that a kernel takes by value.  A tensor that wants a gradient (or carries a tangent) would be taken for one without a word."""
+    if type(value) is float:
+        return value
     if isinstance(value, torch.Tensor):
         wants = torch.is_grad_enabled() and value.requires_grad
         if wants or torch.autograd.forward_ad.unpack_dual(value).tangent is not None:
