@@ -14,8 +14,9 @@
 // (8 elements a lane and step, TPR lanes a row, the next row asked for while one is worked on), its one or two sums go over the
 // lanes by DPP (over LDS beyond a wave), and the column sums of the weight gradients stay in registers over all rows that a block
 // walks; only their block sums go through memory ([blocks][2][D] fp32), joined in a fixed order by a second launch.
-// Measured (copy rate 5.1 TB/s): 16384 x 4096 bf16 forward 92 us (5.8 TB/s, reads past the cache), backward 193 us (4.2); 76800 x 256 fp16 norm
-// alone 12.7 / 27 us; 20000 x 512 fp32 32 / 54 us; 8 x 4096 one launch of 3.8 us.  Rows beyond 8192 columns: backward 2.7 TB/s.
+// Measured (copy rate 5.1 TB/s): 16384 x 4096 bf16 forward 92 us (5.8 TB/s, reads past the cache), backward 191 us (4.2); 76800 x 256 fp16 norm
+// alone 12.7 / 27 us; 20000 x 512 fp32 32 / 54 us; 8 x 4096 one launch of 3.8 us.  Rows beyond 8192 columns: backward 2.6 TB/s.  A gate a token as a
+// gate a channel; a full gate 128 / 253 us (5.2, 4.2 TB/s); a gate for every four rows 123 / 323 us (a block and its two sums for each: 2.9).
 // With a gate per channel (or per sample and channel) S = sum_rows t * nh serves both gradients: dgate = S * post, dpost = sum S * gate.
 #include "token_vec.h"
 

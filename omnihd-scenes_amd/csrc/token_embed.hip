@@ -14,8 +14,9 @@
 //   k_embed_sum   chunks of sorted positions x column slabs: sums each run of equal tokens.  A run inside its chunk is written to the table's
 //                 gradient, a run across chunk borders as fp32 parts to the workspace: work is even however often one token occurs.
 //   k_embed_tail  joins those parts in their order.
-// Measured (copy rate 5.1 TB/s): 65536 x 2048 bf16 of 100000 rows, frequent-word ids: lookup 60 us (5.8 TB/s), gradient 165 us (sort with zero rows
-// 76, sums 73, tail 9; 4.1 TB/s); all ids the same 171 us; 8192 x 1024, fp32 table of 32000 rows: 9 and 42 us; a million ids x 256: 98 and 334 us.
+// Measured (copy rate 5.1 TB/s): 65536 x 2048 bf16 of 100000 rows, frequent-word ids: lookup 59 us (5.9 TB/s), gradient 164 us (sort with zero rows
+// 76, sums 74, tail 9; 4.1 TB/s); all ids the same 171 us; 8192 x 1024, fp32 table of 32000 rows: 8 and 42 us; a million ids x 256: 86 and 332 us (count,
+// offsets and place 46, sort 116, sums 130, tail 44).
 #include "token_vec.h"
 
 namespace omnihd {
@@ -30,6 +31,8 @@ template <typename ID> __device__ __forceinline__ bool usable(ID id, long long v
   return id >= 0 && (long long)id < vocab && (long long)id != padding;
 }
 
+// The output is written past the caches: 65536 x 2048 bf16 of random tokens 75 us, 89 through them.  With the norm that reads it next the two take 180
+// and 183 us there, 43.4 and 41.7 at 32768 x 1024, and as long up to 2048 x 4096 and 8192 x 1024.
 template <typename TT, typename TO, typename ID, int TPR, bool ODD>
 __global__ __launch_bounds__(256) void k_embed_fwd(const ID* __restrict__ ids, const TT* __restrict__ table, long long pitch, long long vocab,
                                                    long long n, int dim, float scale, TO* __restrict__ out) {
@@ -38,7 +41,7 @@ __global__ __launch_bounds__(256) void k_embed_fwd(const ID* __restrict__ ids, c
   for (long long i = (long long)blockIdx.x * RPB + threadIdx.x / TPR; i < n; i += (long long)gridDim.x * RPB) {
     const long long id = (long long)ids[i];
     const bool ok = id >= 0 && id < vocab;
-    for (int c = t * 8; c < dim; c += 4 * TPR * 8) {         // four loads in flight a lane
+    for (int c = t * 8; c < dim; c += 4 * TPR * 8) {         // up to four loads in flight a lane: two in rows up to 4096 columns (fwd)
       float v[4][8];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -51,7 +54,7 @@ __global__ __launch_bounds__(256) void k_embed_fwd(const ID* __restrict__ ids, c
         if (at >= dim) continue;
 #pragma unroll
         for (int k = 0; k < 8; ++k) v[j][k] = ok ? v[j][k] * scale : __builtin_nanf("");
-        store8<ODD, true>(out + i * dim + at, dim - at, v[j]);
+        store8<ODD, true>(out + i * dim + at, dim - at, v[j]);   // past the caches (below)
       }
     }
   }
@@ -441,8 +444,8 @@ int chunk_for(long long n, int dim) {
   while (c < 256 && (n / (2 * c)) * slabs * l >= 4096ll * 64) c *= 2;
   return c;
 }
-// From here on the ids are put into buckets first: three more launches, but no block reads all of them (frequent-word ids, 131072 x 512: 93 us so, 84
-// without; 160000 x 256: 106 us, 143 without; 262144 x 256: 118, 201).
+// From here on the ids are put into buckets first: three more launches, but no block reads all of them (frequent-word ids, 131072 x 512: 102 us so, 92
+// to 119 without; 160000 x 256: 107 us, 147 without; 262144 x 256: 118, 201).
 constexpr long long kBucketIds = 144 << 10;
 int span_for(long long vocab) {
   const long long range = range_for(vocab), ranges = (vocab + range - 1) / range;
@@ -475,7 +478,8 @@ BwdWs bwd_ws(long long n, long long vocab, int dim) {
 
 template <typename TT, typename TO, typename ID, bool ODD>
 int fwd(const void* ids, const void* table, long long pitch, long long vocab, long long n, int dim, float scale, void* out, hipStream_t st) {
-  // two loads a lane and row in flight: 65536 x 2048 bf16 in training 237 us a pass with two, 248 with one, 237 with four (and 64 lanes)
+  // two loads a lane and row in flight: 65536 x 2048 bf16 in training 238 us a pass with two, 247 with one, 236 with four (and 64 lanes); alone 59
+  // with each
   const int tpr = lanes_for((dim + 1) / 2, 256);
   const long long rpb = 256 / tpr, g = (n + rpb - 1) / rpb, most = 64ll * kMaxBlocks;
   const dim3 grid((unsigned)(g < most ? g : most)), block(256);

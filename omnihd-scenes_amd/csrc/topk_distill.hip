@@ -16,7 +16,7 @@
 // The few entries that the teacher names are written again behind the row's own stores, from their own p sums (slots with the same id are
 // summed by the first of them, so an id may stand in a row more than once).
 // Rows of up to 16 entries (the classes of a detection or occupancy head) take a lane each.
-// Measured, loss and gradient (copy rate 5.1 TB/s): 4096 x 131072 bf16 454 us (4.7 TB/s), 4096 x 32000 112 us (4.7), 4096 x 50001 188 us
+// Measured, loss and gradient (copy rate 5.1 TB/s): 4096 x 131072 bf16 453 us (4.7 TB/s), 4096 x 32000 111 us (4.8), 4096 x 50001 185 us
 // (4.4), 60000 x 1000 70 us (3.6: the teacher's part of each row), 614400 x 12 fp32 30 us (2.9: 1000 instructions a wave, half of it arithmetic).
 #include "token_vec.h"
 
@@ -55,7 +55,9 @@ __device__ __forceinline__ typename Pack<T>::V load_pack(const T* __restrict__ p
   for (int k = 0; k < Pack<T>::n; ++k) v[k] = k < left && k >= first ? p[k] : (T)-__builtin_inff();
   return v;
 }
-// (past the caches: the gradient of a large vocabulary is read long after it is written - 1021 x 50021 fp16: 58 us, 49 with it)
+// Past the caches: 1021 x 50021 fp16 44.4 us, 46.2 through them; 2048 x 32000 48 and 51; 614400 x 12 31 and 32.  An operation that reads the gradient
+// at once changes that where the caches would hold it: both together 110 and 95 us at 60000 x 1000, 101 and 95 at 2048 x 32000; 82 each at
+// 1021 x 50021, 42 each at 614400 x 12, 770 each at 4096 x 131072.
 template <bool ODD, typename T>
 __device__ __forceinline__ void store_pack(T* __restrict__ p, int left, const typename Pack<T>::V& v, int first = 0) {
   typedef typename Pack<T>::V V;
@@ -581,7 +583,7 @@ template <typename T> Geometry geometry(int vocab, int top, bool odd) {
   if (packs <= 1024 * 16) return {1024, 16};
   return {1024, 0};
 }
-// (600000 rows of 12 entries, 4 slots: 29 us with a lane a row, 50 with eight; 300000 of 20: 34.5 and 29.6)
+// (600000 rows of 12 entries, 4 slots: 31 us with a lane a row, 53 with eight; 300000 of 20: 33.4 and 29.5, with 12 slots 56 and 40)
 bool by_lanes(int vocab) { return vocab <= kLaneVocab; }
 template <typename T> int blocks_of(long long rows, int vocab, int top, bool odd) {
   if (by_lanes(vocab)) return (int)(rows <= 16384 * 256 ? (rows + 255) / 256 : 16384);
