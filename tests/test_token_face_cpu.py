@@ -41,6 +41,7 @@ def test_dual_tensors_are_refused(call, name, wants, grad):
             CALLS[call][1](face(), m)
 
 
+@pytest.mark.filterwarnings("ignore")                     # (torch's own, about the trace)
 @pytest.mark.parametrize("call,name", NAMED)
 def test_traces_are_refused(call, name):
     """A trace would hold the output's allocation alone."""

@@ -10,6 +10,7 @@ pytestmark = pytest.mark.gpu
 F, B, H = torch.float32, torch.bfloat16, torch.float16
 
 
+@pytest.mark.filterwarnings("ignore")                     # (torch's own, about the trace)
 def test_forward_mode_and_traces_are_refused(cuda):
     """Through the public entry points; beside them, in the same dual level, calls without a tangent run as ever."""
     import torch.autograd.forward_ad as fw
