@@ -246,3 +246,26 @@ def test_occupancy_head_trains_from_a_teacher(cuda, amp):
     check_close(flat(grad), dz, bound(dz, pred.dtype, terms, distill.ROUNDINGS), "gradient")
     for g in torch.autograd.grad(loss, list(student.parameters())):
         assert bool(g.isfinite().all()) and bool(g.any())
+
+
+@pytest.mark.parametrize("dtype", [F, B, H])
+@pytest.mark.parametrize("vocab", [9, 12, 50, 300, 1500, 9001, 40000, 70003, 140001])
+def test_distillation_of_rows_without_a_finite_maximum(cuda, vocab, dtype):
+    """Nothing but -inf, an infinity, a NaN: the row is NaN as its softmax is, unless it has no weight; the rows beside it are what they are alone."""
+    from omnihd_amd import ops
+    z, t, ids, _ = distill.inputs(12, vocab, 4, dtype, F, vocab)
+    inf = float("inf")
+    weight = torch.ones(12, device="cuda")
+    z[1], z[3, vocab // 2], z[5, vocab - 1], z[7], z[8] = -inf, inf, float("nan"), -inf, inf
+    t[9, 1], t[10] = inf, -inf
+    weight[7], weight[8] = 0, 0
+    z.requires_grad_()
+    loss = ops.topk_distill_loss(z, t, ids, row_weight=weight, reduction="none")
+    grad, = torch.autograd.grad(loss, z, torch.ones_like(loss))
+    bad, none, fine = [1, 3, 5, 9], [7, 8, 10], [0, 2, 4, 6, 11]
+    named = torch.zeros(vocab, dtype=torch.bool, device="cuda").index_fill_(0, ids[9], True)     # dz = q - sum of p: p is NaN, q is not
+    assert bool(loss[bad].isnan().all()) and bool(grad[bad[:3]].isnan().all()) and torch.equal(grad[9].isnan(), named)
+    assert not loss[none].any() and not grad[none].any()
+    want, terms, dz, dz_terms = distill.reference(z[fine], t[fine], ids[fine], 1.0, None, 1.0)
+    check_close(loss[fine], want, bound(want, F, terms, distill.ROUNDINGS), "row losses")
+    check_close(grad[fine], dz, bound(dz, dtype, dz_terms, distill.ROUNDINGS) + 2.0 ** -126, "gradient")
